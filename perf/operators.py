@@ -53,8 +53,8 @@ def listed():
         _case("matmul 4096x4096x4096", "matmul", 4096, 4096, 4096),
         # a prompt against a feed-forward projection, hardware scales
         _case("matmul 8192x8192x8192", "matmul", 8192, 8192, 8192, scales="pow2"),
-        # the same in float scales, kept in 32 bits for what follows
-        _case("matmul 4096x10240x4096 fp32", "matmul", 4096, 10240, 4096, dtype="fp32"),
+        # a wide projection of a prompt in float scales; fp16 out
+        _case("matmul 4096x10240x4096 fp16", "matmul", 4096, 10240, 4096, dtype="fp16"),
     ]
 
 
@@ -71,6 +71,7 @@ def draw(rng):
     c = {"op": op, "dtype": rng.choice(["bf16", "bf16", "fp16", "fp32"]), "scales": rng.choice(["float", "pow2"]),
          "residual": False, "block_rows": 1, "bias": False, "inner": 0}
     if op == "matmul":
+        c["dtype"] = rng.choice(["bf16", "fp16"])         # sums of 8-bit products are handed on in 16 bits
         c["cols"] = _spread(rng, 16, 16384)
         c["inner"] = _spread(rng, 64, 16384)
         c["rows"] = _spread(rng, 1, min(16384, 8192 ** 3 // (c["cols"] * c["inner"])))
