@@ -1,0 +1,86 @@
+"""The 8-bit operators' checks of their arguments and the block matrix's layouts (no GPU)."""
+import pytest
+import torch
+
+from yoda_scheduler_amd.ops import fp8
+from yoda_scheduler_amd.ops.fp8 import BLOCK, E4M3, E8M0, BlockMatrix
+
+
+def _matrix(rows, cols, block_rows=1, scale_dtype=torch.float32):
+    kb = fp8.blocks(cols)
+    return BlockMatrix(torch.zeros(rows, kb * BLOCK).to(E4M3),
+                       torch.ones(rows if block_rows == 1 else fp8.blocks(rows), kb).to(scale_dtype), cols, block_rows)
+
+
+def test_unpadded_values_are_padded_with_zeros_and_scales_laid_out():
+    v = torch.arange(3 * 130, dtype=torch.float32).view(3, 130).fmod(9).to(E4M3)
+    s = torch.tensor([[1.0, 2.0], [3.0, 4.0], [5.0, 6.0]])
+    m = BlockMatrix(v, s)
+    assert m.shape == (3, 130) and m.data.shape == (3, 256) and m.values.shape == (3, 130)
+    assert torch.equal(m.values.float(), v.float())
+    assert torch.equal(m.data[:, 130:].float(), torch.zeros(3, 126))
+    assert m.scales.t().is_contiguous() and torch.equal(m.scales, s)
+    w = BlockMatrix(v, torch.tensor([[2.0, 0.5]]).to(E8M0), block_rows=128)
+    assert w.scales.is_contiguous() and w.scales.shape == (1, 2)
+    assert "3x130" in repr(w)
+
+
+def test_padded_values_are_taken_as_they_are():
+    v = torch.zeros(5, 256).to(E4M3)
+    s = torch.ones(2, 5).t()
+    m = BlockMatrix(v, s, cols=200)
+    assert m.data.data_ptr() == v.data_ptr() and m.scales.data_ptr() == s.data_ptr() and m.cols == 200
+
+
+@pytest.mark.parametrize("values,scales,kw,error", [
+    (torch.zeros(4, 128), torch.ones(4, 1), {}, TypeError),                                   # not e4m3
+    (torch.zeros(128).to(E4M3), torch.ones(1, 1), {}, TypeError),                             # one axis
+    (torch.zeros(4, 128).to(E4M3), torch.ones(4, 1, dtype=torch.float64), {}, TypeError),     # scales' type
+    (torch.zeros(4, 128).to(E4M3), torch.ones(4), {}, TypeError),
+    (torch.zeros(4, 128).to(E4M3), torch.ones(4, 2), {}, ValueError),                         # scales' shape
+    (torch.zeros(4, 128).to(E4M3), torch.ones(4, 1), {"block_rows": 128}, ValueError),
+    (torch.zeros(4, 128).to(E4M3), torch.ones(4, 1), {"block_rows": 64}, ValueError),
+    (torch.zeros(4, 256).to(E4M3), torch.ones(4, 1), {"cols": 100}, ValueError),              # padded too far
+    (torch.zeros(4, 0).to(E4M3), torch.ones(4, 0), {}, ValueError),
+    (torch.zeros(4, 128).to(E4M3), torch.ones(4, 1, device="meta"), {}, ValueError),          # another device
+])
+def test_block_matrix_refuses(values, scales, kw, error):
+    with pytest.raises(error):
+        BlockMatrix(values, scales, **kw)
+
+
+@pytest.mark.parametrize("x,kw,error", [
+    (torch.zeros(4, 128), {}, ValueError),                                                    # not on a GPU
+    (torch.zeros(4, 128, dtype=torch.float64), {}, TypeError),
+    (torch.zeros(4, 128, dtype=torch.int8), {}, TypeError),
+    (torch.zeros(128), {}, ValueError),
+    (torch.zeros(2, 4, 128), {}, ValueError),
+    (torch.zeros(128, 4).t(), {}, ValueError),                                                # columns apart
+])
+def test_quantize_and_norm_refuse(x, kw, error):
+    with pytest.raises(error):
+        fp8.quantize(x, **kw)
+    with pytest.raises(error):
+        fp8.add_rms_norm(x, torch.ones(x.shape[-1], dtype=x.dtype), **kw)
+
+
+def test_scale_dtype_and_gradients_are_refused():
+    with pytest.raises(TypeError):
+        fp8._scale_kind(torch.float16)
+    w = torch.ones(4, requires_grad=True)
+    with pytest.raises(RuntimeError):
+        fp8._no_grad(None, w)
+    with torch.no_grad():
+        fp8._no_grad(w)
+
+
+@pytest.mark.parametrize("a,b,kw,error", [
+    (_matrix(4, 128, 128), _matrix(4, 128, 128), {}, ValueError),                             # a's blocks
+    (_matrix(4, 128), _matrix(4, 128), {}, ValueError),                                       # b's blocks
+    (_matrix(4, 128), _matrix(4, 129, 128), {}, ValueError),                                  # columns
+    (_matrix(4, 128), _matrix(4, 128, 128, E8M0), {}, TypeError),                             # two kinds of scales
+    (_matrix(4, 128), _matrix(4, 128, 128), {}, ValueError),                                  # not on a GPU
+])
+def test_matmul_refuses(a, b, kw, error):
+    with pytest.raises(error):
+        fp8.matmul(a, b, **kw)

@@ -68,7 +68,7 @@ ARTEFACTS: dict[str, dict] = {
                              "common/build_id.h"],
                     "recipe": "g++ -O2 -std=c++17 -lamd_smi v2"},
     "hip": {"out": "libyoda_hip.so", "srcs": None, "deps": None,     # every native/hip/*.hip + *.h
-            "recipe": f"hipcc --offload-arch={ARCH} -O3 -std=c++17 -fPIC -shared v2"},
+            "recipe": f"hipcc --offload-arch={ARCH} -O3 -std=c++17 -fPIC -shared -packed-fp32-ops v3"},
 }
 
 
@@ -213,7 +213,9 @@ def build_hip(force: bool = False) -> Path:
     out = out_path("hip")
     if force or _stale("hip"):
         bid = source_hash("hip")
+        # no packed float32 instructions: some of their forms have given wrong results on MI355X
         _run([hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared", _bid_flag(bid),
+              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
               "-Wall", "-Wno-unused-result", "-Wno-unused-value", f"-I{src}", f"-I{NATIVE / 'common'}",
               *map(str, srcs), "-o", str(out)], "hip kernels")
         _record("hip", bid)

@@ -22,9 +22,9 @@ _lock = threading.Lock()
 # YODA_HIP_LIB points at another build of the kernels (same-box A/B of kernel variants)
 PATH = Path(os.environ.get("YODA_HIP_LIB") or Path(__file__).resolve().parents[1] / "_native" / "libyoda_hip.so")
 
-c_int, c_uint, c_ull, c_double, c_float, c_char_p, c_void_p = (
-    ctypes.c_int, ctypes.c_uint, ctypes.c_ulonglong, ctypes.c_double, ctypes.c_float, ctypes.c_char_p,
-    ctypes.c_void_p)
+c_int, c_uint, c_ull, c_int64, c_double, c_float, c_char_p, c_void_p = (
+    ctypes.c_int, ctypes.c_uint, ctypes.c_ulonglong, ctypes.c_int64, ctypes.c_double, ctypes.c_float,
+    ctypes.c_char_p, ctypes.c_void_p)
 
 
 class HipError(RuntimeError):
@@ -43,9 +43,20 @@ def _declare(lib: ctypes.CDLL) -> None:
         "yoda_peer_write_bandwidth": [c_int, c_int, c_ull, c_int, P(c_double), P(c_int)],
         "yoda_hip_occupy": [c_int, c_int, P(c_int)],
         "yoda_hip_occupy_wait": [c_int],
+        # ops/fp8.py: device, stream, types and switches, tensors, sizes
+        "yoda_fp8_norm": [c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                          c_void_p, c_void_p, c_void_p, c_int64, c_int, c_float],
+        "yoda_fp8_quantize": [c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                              c_int],
+        "yoda_fp8_matmul": [c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                            c_int64, c_int64, c_int, c_int64],
     }
     for name, args in sigs.items():
-        f = getattr(lib, name)
+        f = getattr(lib, name, None)
+        if f is None and name.startswith("yoda_fp8_"):
+            continue                      # another build of the probes (YODA_HIP_LIB) may lack the operators
+        if f is None:
+            raise AttributeError(f"{PATH} has no {name}")
         f.argtypes = args
         f.restype = c_int
     try:
