@@ -19,6 +19,19 @@ struct MatArgs {
   int kb;                              // Kp / 128
 };
 
+template <int I>
+struct Index {
+  static constexpr int value = I;
+};
+// f(0), f(1), ... f(N - 1) with their numbers known to the compiler
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void each(F& f) {
+  if constexpr (I < N) {
+    f(Index<I>{});
+    each<N, I + 1>(f);
+  }
+}
+
 __device__ __forceinline__ i32x8 load32(const uint8_t* p) {
   const i32x4 x = *(const i32x4*)p, y = *(const i32x4*)(p + 16);
   return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -63,14 +76,259 @@ __global__ __launch_bounds__(256) void k_simple(MatArgs p) {
   }
 }
 
+// ---------------------------------------------------------------- tiles through LDS
+//
+// One workgroup a tile of BM x BN, 128 of K a step: each wave holds 16*MT rows m times 16*NT columns
+// n of sums. Rows and columns are dealt to the lanes so that what belongs to a lane lies together:
+// lane (c, g) = (lane % 16, lane / 16) has the rows m = c*MT + i of its wave (i < MT: one load brings
+// its scales) and the columns n = g*4*NT + 4*j + r (j < NT, r < 4: it stores 4*NT neighbours).
+//
+// Both tiles lie in LDS as rows of 128 bytes, their eight 16-byte pieces exchanged by
+// piece ^= key(row), key = the low three bits of the c that reads the row, so that eight lanes which
+// read a piece of eight rows at once meet eight different bank groups. The loads go from memory into LDS
+// directly: lane l of a load fills piece l % 8 of row l / 8, and takes the piece of memory that
+// belongs there.
+template <int MT_, int NT_, int WM_, int WN_>
+struct Tile {
+  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_;
+  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN;
+  static constexpr int kBytes = (BM + BN) * kBlockK;              // one step of both tiles
+  static constexpr int kLoadsA = BM / 8 / kWaves, kLoadsB = BN / 8 / kWaves;   // 1024-byte loads of a wave
+  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "whole loads for every wave");
+};
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+// Lane l's 16 bytes at base + voff + soff go to LDS at lds + 16 l.
+__device__ __forceinline__ void load_lds(u32x4 rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
+               : "memory");
+}
+
+__device__ __forceinline__ u32x4 buffer_of(const void* base) {
+  const uint64_t at = (uint64_t)base;
+  u32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((uint32_t)at);
+  r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+  r[2] = 0xFFFFFFFFu;
+  r[3] = 0x00020000u;
+  return r;
+}
+
+// MT scales of a lane's rows m .. m + MT - 1 of one block along K, as they are held.
+template <bool POW2, int MT>
+struct Scales {
+  float f[POW2 ? 1 : MT];
+  uint32_t b[POW2 ? MT / 4 : 1];
+  // whole: every row exists
+  __device__ __forceinline__ void load(const void* base, int64_t rows, int64_t kb, int64_t m, bool whole) {
+    if constexpr (POW2) {
+      const uint8_t* p = (const uint8_t*)base + kb * rows;
+      struct __attribute__((packed, aligned(1))) Bytes { uint32_t w[MT / 4]; };
+      if (whole) {
+        const Bytes x = *(const Bytes*)(p + m);
+#pragma unroll
+        for (int i = 0; i < MT / 4; ++i) b[i] = x.w[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < MT / 4; ++i) {
+          b[i] = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) b[i] |= (uint32_t)p[m + 4 * i + k < rows ? m + 4 * i + k : rows - 1] << (8 * k);
+        }
+      }
+    } else {
+      const float* p = (const float*)base + kb * rows;
+      struct __attribute__((packed, aligned(4))) Floats { float w[MT]; };
+      if (whole) {
+        const Floats x = *(const Floats*)(p + m);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) f[i] = x.w[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) f[i] = p[m + i < rows ? m + i : rows - 1];
+      }
+    }
+  }
+  // The loads have arrived (and are not waited for again behind later ones).
+  __device__ __forceinline__ void arrived() {
+    if constexpr (POW2) {
+#pragma unroll
+      for (int i = 0; i < MT / 4; ++i) asm volatile("" : "+v"(b[i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(f[i]));
+    }
+  }
+};
+
+template <bool POW2, int I>
+__device__ __forceinline__ f32x4 mfma_scaled(i32x8 w, i32x8 x, f32x4 acc, uint32_t wscale, uint32_t xscales) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc, 0, 0, 0, (int)wscale, I, (int)xscales);
+}
+
+template <typename T, typename O, bool POW2>
+__global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 2 : 1) void k_tile(MatArgs p, int tiles_m, int tiles_n) {
+  constexpr int MT = T::MT, NT = T::NT;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * T::kBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4, wm = wave / T::WN, wn = wave % T::WN;
+
+  // tiles: each XCD a run of them, in columns of kGroup rows, so that what runs at one time shares rows and columns
+  constexpr int kXcds = 8, kGroup = 4;
+  int tm, tn;
+  {
+    const int total = tiles_m * tiles_n, run = (total + kXcds - 1) / kXcds;
+    const int at = blockIdx.x / kXcds, t = (blockIdx.x % kXcds) * run + at;
+    if (at >= run || t >= total) return;
+    const int per = kGroup * tiles_n, first = t / per * kGroup, rows = min(kGroup, tiles_m - first);
+    tm = first + t % per % rows;
+    tn = t % per / rows;
+  }
+  const int64_t m0 = (int64_t)tm * T::BM, n0 = (int64_t)tn * T::BN, kp = (int64_t)p.kb * kBlockK;
+
+  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  const u32x4 ra = buffer_of(p.a + m0 * kp), rb = buffer_of(p.b + n0 * kp);
+  uint32_t va[T::kLoadsA], vb[T::kLoadsB];
+#pragma unroll
+  for (int i = 0; i < T::kLoadsA; ++i) {
+    const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = row / MT & 7;
+    const int64_t in = m0 + row < p.m ? row : p.m - 1 - m0;
+    va[i] = (uint32_t)(in * kp + ((lane & 7) ^ key) * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < T::kLoadsB; ++i) {
+    const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = (row & 3) | (row / (4 * NT) & 1) << 2;
+    const int64_t in = n0 + row < p.n ? row : p.n - 1 - n0;
+    vb[i] = (uint32_t)(in * kp + ((lane & 7) ^ key) * 16);
+  }
+  auto fetch = [&](int kb, int buf) {
+    const uint32_t to = base + buf * T::kBytes;
+#pragma unroll
+    for (int i = 0; i < T::kLoadsA; ++i) load_lds(ra, va[i], kb * kBlockK, to + (wave + i * T::kWaves) * 1024);
+#pragma unroll
+    for (int i = 0; i < T::kLoadsB; ++i)
+      load_lds(rb, vb[i], kb * kBlockK, to + T::BM * kBlockK + (wave + i * T::kWaves) * 1024);
+  };
+
+  const int64_t m = m0 + wm * 16 * MT + c * MT, n = n0 + wn * 16 * NT + g * 4 * NT;
+  const bool whole = m0 + T::BM <= p.m;
+  const int64_t sb_at = min(n0 + wn * 16 * NT, p.n - 1) / kBlockK * p.kb;
+  Scales<POW2, MT> sa;
+  float sb_f = 0.f;
+  uint32_t sb_b = 0;
+  auto scales = [&](int kb) {
+    sa.load(p.sa, p.m, kb, m, whole);
+    if constexpr (POW2) sb_b = ((const uint8_t*)p.sb)[sb_at + kb];
+    else sb_f = ((const float*)p.sb)[sb_at + kb];
+  };
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const uint8_t* la = lds + (wm * 16 * MT + c * MT) * kBlockK;
+  const uint8_t* lb = lds + T::BM * kBlockK + (wn * 16 * NT + (c >> 2) * 4 * NT + (c & 3)) * kBlockK;
+  const int piece0 = (g ^ (c & 7)) * 16, piece1 = piece0 ^ 64;
+
+  fetch(0, 0);
+  scales(0);
+  for (int kb = 0; kb < p.kb; ++kb) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    sa.arrived();
+    Scales<POW2, MT> now = sa;
+    const float wf = sb_f;
+    const uint32_t wb = sb_b;
+    if (kb + 1 < p.kb) {
+      scales(kb + 1);
+      fetch(kb + 1, (kb + 1) & 1);
+    }
+    const int buf = (kb & 1) * T::kBytes;
+    i32x8 w[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const i32x4 x = *(const i32x4*)(lb + buf + j * 4 * kBlockK + piece0);
+      const i32x4 y = *(const i32x4*)(lb + buf + j * 4 * kBlockK + piece1);
+      w[j] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    auto row = [&](auto I) {
+      constexpr int i = decltype(I)::value;
+      const i32x4 x = *(const i32x4*)(la + buf + i * kBlockK + piece0);
+      const i32x4 y = *(const i32x4*)(la + buf + i * kBlockK + piece1);
+      const i32x8 v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if constexpr (POW2) {
+          acc[i][j] = mfma_scaled<POW2, i & 3>(w[j], v, acc[i][j], wb, now.b[i >> 2]);
+        } else {
+          const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+          const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[j], v, zero, 0, 0, 0, 0, 0, 0);
+          const float s = now.f[i] * wf;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[r], s, acc[i][j][r]);
+        }
+      }
+    };
+    each<MT>(row);
+  }
+
+  using B = typename Bits<O>::type;
+  float bias[NT * 4];
+#pragma unroll
+  for (int k = 0; k < NT * 4; ++k) bias[k] = p.bias && n + k < p.n ? load_f32<O>(((const B*)p.bias)[n + k]) : 0.f;
+  struct __attribute__((packed, aligned(sizeof(B)))) Out { B b[NT * 4]; };
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    if (m + i >= p.m) break;
+    Out o;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o.b[4 * j + r] = store_bits<O>(acc[i][j][r] + bias[4 * j + r]);
+    B* to = (B*)p.out + (m + i) * p.pitch + n;
+    if (n + NT * 4 <= p.n) {
+      *(Out*)to = o;
+    } else {
+#pragma unroll
+      for (int k = 0; k < NT * 4; ++k)
+        if (n + k < p.n) to[k] = o.b[k];
+    }
+  }
+}
+
+template <typename T, typename O>
+int run_tile(const MatArgs& p, bool pow2, hipStream_t s) {
+  const int64_t tm = (p.m + T::BM - 1) / T::BM, tn = (p.n + T::BN - 1) / T::BN, total = tm * tn;
+  if (total > (1 << 30)) return -1;
+  const unsigned grid = (unsigned)((total + 7) / 8 * 8);
+  if (pow2) k_tile<T, O, true><<<grid, T::kThreads, 0, s>>>(p, (int)tm, (int)tn);
+  else k_tile<T, O, false><<<grid, T::kThreads, 0, s>>>(p, (int)tm, (int)tn);
+  return (int)hipGetLastError();
+}
+
+using Big = Tile<8, 4, 2, 4>;
+
 template <typename O>
-int run(const MatArgs& p, bool pow2, hipStream_t s) {
+int run_simple(const MatArgs& p, bool pow2, hipStream_t s) {
   const int64_t gx = (p.n + 63) / 64, gy = (p.m + 15) / 16;
   if (gx > 0x7FFFFFFF || gy > 65535) return -1;
   const dim3 grid((unsigned)gx, (unsigned)gy);
   if (pow2) k_simple<O, true><<<grid, 256, 0, s>>>(p);
   else k_simple<O, false><<<grid, 256, 0, s>>>(p);
   return (int)hipGetLastError();
+}
+
+template <typename O>
+int run(const MatArgs& p, bool pow2, hipStream_t s) {
+  if (p.m > 64) return run_tile<Big, O>(p, pow2, s);
+  return run_simple<O>(p, pow2, s);
 }
 
 }  // namespace
@@ -84,7 +342,7 @@ extern "C" {
 // arguments out of range.
 int yoda_fp8_matmul(int device, void* stream, int out_type, int pow2, const void* a, const void* sa, const void* b,
                     const void* sb, const void* bias, void* out, int64_t m, int64_t n, int kb, int64_t pitch) {
-  if ((out_type != kBf16 && out_type != kFp16) || m < 0 || n < 0 || kb < 1 || kb > (1 << 23) || pitch < n) return -1;
+  if ((out_type != kBf16 && out_type != kFp16) || m < 0 || n < 0 || kb < 1 || kb > 65535 || pitch < n) return -1;
   if (m == 0 || n == 0) return 0;
   if (!a || !sa || !b || !sb || !out) return -1;
   DeviceScope on(device);
