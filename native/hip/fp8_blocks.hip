@@ -126,7 +126,7 @@ __device__ __forceinline__ int64_t row_of(int64_t b, int64_t rows) {
 struct NormArgs {
   const void *x, *residual, *weight;
   void *stream_out, *values, *scales;
-  int64_t rows, x_pitch, r_pitch;      // pitches in elements
+  int64_t rows, x_pitch, r_pitch, s_pitch;   // pitches in elements
   int cols, padded;
   float eps;
 };
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
       }
       const float s = scale_of<POW2>(row_max(amax));
       *(uint2*)(q + c) = to_e4m3(y, __fdiv_rn(1.f, s));
-      if (tid % kLanes == 0) put_scale<POW2>(a.scales, (int64_t)(c / kBlockK) * a.rows + r, s);
+      if (tid % kLanes == 0) put_scale<POW2>(a.scales, (int64_t)(c / kBlockK) * a.s_pitch + r, s);
     }
   }
 }
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
 struct QuantArgs {
   const void* x;
   void *values, *scales;
-  int64_t rows, pitch;
+  int64_t rows, pitch, s_pitch;
   int cols, padded, lane_bits;         // 1 << lane_bits lanes a row and pass
 };
 
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void k_rows(QuantArgs a) {
     for (int i = 0; i < kWidth; ++i) amax = fmaxf(amax, finite_abs(v[i]));
     const float s = scale_of<POW2>(row_max(amax));
     *(uint2*)(q + c) = to_e4m3(v, __fdiv_rn(1.f, s));
-    if (threadIdx.x % kLanes == 0) put_scale<POW2>(a.scales, (int64_t)(c / kBlockK) * a.rows + r, s);
+    if (threadIdx.x % kLanes == 0) put_scale<POW2>(a.scales, (int64_t)(c / kBlockK) * a.s_pitch + r, s);
   }
 }
 
@@ -335,7 +335,8 @@ int yoda_fp8_norm(int device, void* stream, int type, int weight_f32, int pow2, 
   if (!x || !weight || !values || !scales) return -1;
   DeviceScope on(device);
   if (on.err != hipSuccess) return (int)on.err;
-  const NormArgs a = {x, residual, weight, stream_out, values, scales, rows, x_pitch, r_pitch, cols, padded_cols(cols), eps};
+  const NormArgs a = {x, residual, weight, stream_out, values, scales, rows, x_pitch, r_pitch, (rows + 7) / 8 * 8, cols,
+                      padded_cols(cols), eps};
   const hipStream_t s = (hipStream_t)stream;
   if (type == kFp32) return norm_typed<float, float>(a, pow2, s);
   if (type == kFp16) return weight_f32 ? norm_typed<__half, float>(a, pow2, s) : norm_typed<__half, __half>(a, pow2, s);
@@ -351,7 +352,7 @@ int yoda_fp8_quantize(int device, void* stream, int type, int tiles, int pow2, c
   if (!x || !values || !scales) return -1;
   DeviceScope on(device);
   if (on.err != hipSuccess) return (int)on.err;
-  QuantArgs a = {x, values, scales, rows, pitch, cols, padded_cols(cols), 4};
+  QuantArgs a = {x, values, scales, rows, pitch, (rows + 7) / 8 * 8, cols, padded_cols(cols), 4};
   while (a.lane_bits < 8 && (kWidth << a.lane_bits) < a.padded) ++a.lane_bits;
   const hipStream_t s = (hipStream_t)stream;
   if (type == kFp32) return quant_typed<float>(a, tiles, pow2, s);

@@ -12,10 +12,10 @@ namespace {
 
 struct MatArgs {
   const uint8_t *a, *b;                // [M][Kp], [N][Kp]
-  const void *sa, *sb;                 // [Kp/128][M], [ceil(N/128)][Kp/128]
+  const void *sa, *sb;                 // [Kp/128][sa_pitch], [ceil(N/128)][Kp/128]
   const void* bias;                    // [N] of the output's type, or null
   void* out;
-  int64_t m, n, pitch;                 // pitch of out in elements
+  int64_t m, n, pitch, sa_pitch;       // pitch of out in elements; sa_pitch: m up to a multiple of 8
   int kb;                              // Kp / 128
 };
 
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void k_simple(MatArgs p) {
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(load32(b + kb * kBlockK), load32(a + kb * kBlockK),
                                                                     zero, 0, 0, 0, 0, 0, 0);
-    const float s = scale_at<POW2>(p.sa, (int64_t)kb * p.m + am) * scale_at<POW2>(p.sb, n0 / kBlockK * p.kb + kb);
+    const float s = scale_at<POW2>(p.sa, (int64_t)kb * p.sa_pitch + am) * scale_at<POW2>(p.sb, n0 / kBlockK * p.kb + kb);
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = fmaf(t[i], s, acc[i]);
   }
@@ -118,167 +118,97 @@ __device__ __forceinline__ u32x4 buffer_of(const void* base) {
   return r;
 }
 
-// MT scales of a lane's rows m .. m + MT - 1 of one block along K, as they are held.
-template <bool POW2, int MT>
+// Eight scales of a lane's rows m .. m + 7 of one block along K, as they are held. m is a multiple of 8 and
+// below the pitch, which is one too.
+template <bool POW2>
 struct Scales {
-  float f[POW2 ? 1 : MT];
-  uint32_t b[POW2 ? MT / 4 : 1];
-  // whole: every row exists
-  __device__ __forceinline__ void load(const void* base, int64_t rows, int64_t kb, int64_t m, bool whole) {
+  float f[POW2 ? 1 : 8];
+  uint32_t b[POW2 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* base, int64_t at) {
     if constexpr (POW2) {
-      const uint8_t* p = (const uint8_t*)base + kb * rows;
-      struct __attribute__((packed, aligned(1))) Bytes { uint32_t w[MT / 4]; };
-      if (whole) {
-        const Bytes x = *(const Bytes*)(p + m);
-#pragma unroll
-        for (int i = 0; i < MT / 4; ++i) b[i] = x.w[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < MT / 4; ++i) {
-          b[i] = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) b[i] |= (uint32_t)p[m + 4 * i + k < rows ? m + 4 * i + k : rows - 1] << (8 * k);
-        }
-      }
+      const uint2 x = *(const uint2*)((const uint8_t*)base + at);
+      b[0] = x.x, b[1] = x.y;
     } else {
-      const float* p = (const float*)base + kb * rows;
-      struct __attribute__((packed, aligned(4))) Floats { float w[MT]; };
-      if (whole) {
-        const Floats x = *(const Floats*)(p + m);
+      const f32x4 *x = (const f32x4*)((const float*)base + at), u = x[0], v = x[1];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) f[i] = x.w[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < MT; ++i) f[i] = p[m + i < rows ? m + i : rows - 1];
-      }
+      for (int i = 0; i < 4; ++i) f[i] = u[i], f[4 + i] = v[i];
     }
   }
   // The loads have arrived (and are not waited for again behind later ones).
   __device__ __forceinline__ void arrived() {
     if constexpr (POW2) {
-#pragma unroll
-      for (int i = 0; i < MT / 4; ++i) asm volatile("" : "+v"(b[i]));
+      asm volatile("" : "+v"(b[0]), "+v"(b[1]));
     } else {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(f[i]));
+      for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(f[i]));
     }
   }
 };
 
-template <bool POW2, int I>
+__device__ __forceinline__ i32x8 join(const i32x4 (&v)[2]) {
+  return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// I: which byte of xscales holds this piece's scale
+template <int I>
 __device__ __forceinline__ f32x4 mfma_scaled(i32x8 w, i32x8 x, f32x4 acc, uint32_t wscale, uint32_t xscales) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc, 0, 0, 0, (int)wscale, I, (int)xscales);
 }
 
-template <typename T, typename O, bool POW2>
-__global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 2 : 1) void k_tile(MatArgs p, int tiles_m, int tiles_n) {
-  constexpr int MT = T::MT, NT = T::NT;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * T::kBytes];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4, wm = wave / T::WN, wn = wave % T::WN;
-
-  // tiles: each XCD a run of them, in columns of kGroup rows, so that what runs at one time shares rows and columns
+// The tile of a workgroup: each XCD gets a run of them, in columns of kGroup rows, so that what runs at one
+// time on an XCD shares rows and columns in its L2. False past the end.
+__device__ __forceinline__ bool tile_of(int block, int tiles_m, int tiles_n, int& tm, int& tn) {
   constexpr int kXcds = 8, kGroup = 4;
-  int tm, tn;
-  {
-    const int total = tiles_m * tiles_n, run = (total + kXcds - 1) / kXcds;
-    const int at = blockIdx.x / kXcds, t = (blockIdx.x % kXcds) * run + at;
-    if (at >= run || t >= total) return;
-    const int per = kGroup * tiles_n, first = t / per * kGroup, rows = min(kGroup, tiles_m - first);
-    tm = first + t % per % rows;
-    tn = t % per / rows;
-  }
-  const int64_t m0 = (int64_t)tm * T::BM, n0 = (int64_t)tn * T::BN, kp = (int64_t)p.kb * kBlockK;
+  const int total = tiles_m * tiles_n, run = (total + kXcds - 1) / kXcds;
+  const int at = block / kXcds, t = (block % kXcds) * run + at;
+  if (at >= run || t >= total) return false;
+  const int per = kGroup * tiles_n, first = t / per * kGroup, rows = min(kGroup, tiles_m - first);
+  tm = first + t % per % rows;
+  tn = t % per / rows;
+  return true;
+}
 
-  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  const u32x4 ra = buffer_of(p.a + m0 * kp), rb = buffer_of(p.b + n0 * kp);
-  uint32_t va[T::kLoadsA], vb[T::kLoadsB];
+// A wave's share of the loads of both tiles' steps into LDS. Rows past the end repeat the last one.
+template <typename T>
+struct Loader {
+  u32x4 ra, rb;
+  uint32_t va[T::kLoadsA], vb[T::kLoadsB], base;
+  int wave;
+  __device__ __forceinline__ Loader(const MatArgs& p, uint8_t* lds, int64_t m0, int64_t n0, int wave_, int lane)
+      : wave(wave_) {
+    const int64_t kp = (int64_t)p.kb * kBlockK;
+    base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    ra = buffer_of(p.a + m0 * kp);
+    rb = buffer_of(p.b + n0 * kp);
 #pragma unroll
-  for (int i = 0; i < T::kLoadsA; ++i) {
-    const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = row / MT & 7;
-    const int64_t in = m0 + row < p.m ? row : p.m - 1 - m0;
-    va[i] = (uint32_t)(in * kp + ((lane & 7) ^ key) * 16);
-  }
+    for (int i = 0; i < T::kLoadsA; ++i) {
+      const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = row / T::MT & 7;
+      const int64_t in = m0 + row < p.m ? row : p.m - 1 - m0;
+      va[i] = (uint32_t)(in * kp + ((lane & 7) ^ key) * 16);
+    }
 #pragma unroll
-  for (int i = 0; i < T::kLoadsB; ++i) {
-    const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = (row & 3) | (row / (4 * NT) & 1) << 2;
-    const int64_t in = n0 + row < p.n ? row : p.n - 1 - n0;
-    vb[i] = (uint32_t)(in * kp + ((lane & 7) ^ key) * 16);
+    for (int i = 0; i < T::kLoadsB; ++i) {
+      const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = (row & 3) | (row / (4 * T::NT) & 1) << 2;
+      const int64_t in = n0 + row < p.n ? row : p.n - 1 - n0;
+      vb[i] = (uint32_t)(in * kp + ((lane & 7) ^ key) * 16);
+    }
   }
-  auto fetch = [&](int kb, int buf) {
+  // load i of the step's kLoadsA + kLoadsB
+  __device__ __forceinline__ void one(int i, int kb, int buf) {
     const uint32_t to = base + buf * T::kBytes;
-#pragma unroll
-    for (int i = 0; i < T::kLoadsA; ++i) load_lds(ra, va[i], kb * kBlockK, to + (wave + i * T::kWaves) * 1024);
-#pragma unroll
-    for (int i = 0; i < T::kLoadsB; ++i)
-      load_lds(rb, vb[i], kb * kBlockK, to + T::BM * kBlockK + (wave + i * T::kWaves) * 1024);
-  };
-
-  const int64_t m = m0 + wm * 16 * MT + c * MT, n = n0 + wn * 16 * NT + g * 4 * NT;
-  const bool whole = m0 + T::BM <= p.m;
-  const int64_t sb_at = min(n0 + wn * 16 * NT, p.n - 1) / kBlockK * p.kb;
-  Scales<POW2, MT> sa;
-  float sb_f = 0.f;
-  uint32_t sb_b = 0;
-  auto scales = [&](int kb) {
-    sa.load(p.sa, p.m, kb, m, whole);
-    if constexpr (POW2) sb_b = ((const uint8_t*)p.sb)[sb_at + kb];
-    else sb_f = ((const float*)p.sb)[sb_at + kb];
-  };
-
-  f32x4 acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const uint8_t* la = lds + (wm * 16 * MT + c * MT) * kBlockK;
-  const uint8_t* lb = lds + T::BM * kBlockK + (wn * 16 * NT + (c >> 2) * 4 * NT + (c & 3)) * kBlockK;
-  const int piece0 = (g ^ (c & 7)) * 16, piece1 = piece0 ^ 64;
-
-  fetch(0, 0);
-  scales(0);
-  for (int kb = 0; kb < p.kb; ++kb) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    sa.arrived();
-    Scales<POW2, MT> now = sa;
-    const float wf = sb_f;
-    const uint32_t wb = sb_b;
-    if (kb + 1 < p.kb) {
-      scales(kb + 1);
-      fetch(kb + 1, (kb + 1) & 1);
-    }
-    const int buf = (kb & 1) * T::kBytes;
-    i32x8 w[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const i32x4 x = *(const i32x4*)(lb + buf + j * 4 * kBlockK + piece0);
-      const i32x4 y = *(const i32x4*)(lb + buf + j * 4 * kBlockK + piece1);
-      w[j] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-    auto row = [&](auto I) {
-      constexpr int i = decltype(I)::value;
-      const i32x4 x = *(const i32x4*)(la + buf + i * kBlockK + piece0);
-      const i32x4 y = *(const i32x4*)(la + buf + i * kBlockK + piece1);
-      const i32x8 v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        if constexpr (POW2) {
-          acc[i][j] = mfma_scaled<POW2, i & 3>(w[j], v, acc[i][j], wb, now.b[i >> 2]);
-        } else {
-          const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-          const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[j], v, zero, 0, 0, 0, 0, 0, 0);
-          const float s = now.f[i] * wf;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[r], s, acc[i][j][r]);
-        }
-      }
-    };
-    each<MT>(row);
+    if (i < T::kLoadsA)
+      load_lds(ra, va[i], kb * kBlockK, to + (wave + i * T::kWaves) * 1024);
+    else
+      load_lds(rb, vb[i - T::kLoadsA], kb * kBlockK, to + T::BM * kBlockK + (wave + (i - T::kLoadsA) * T::kWaves) * 1024);
   }
+  __device__ __forceinline__ void fetch(int kb, int buf) {
+#pragma unroll
+    for (int i = 0; i < T::kLoadsA + T::kLoadsB; ++i) one(i, kb, buf);
+  }
+};
 
+template <int MT, int NT, typename O>
+__device__ __forceinline__ void store_tile(const MatArgs& p, const f32x4 (&acc)[MT][NT], int64_t m, int64_t n) {
   using B = typename Bits<O>::type;
   float bias[NT * 4];
 #pragma unroll
@@ -303,6 +233,184 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 2 : 1) void k_til
   }
 }
 
+template <typename T, typename O, bool POW2>
+__global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 2 : 1) void k_tile(MatArgs p, int tiles_m, int tiles_n) {
+  constexpr int MT = T::MT, NT = T::NT;
+  static_assert(MT == 8, "a lane's rows have one load of scales");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * T::kBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4, wm = wave / T::WN, wn = wave % T::WN;
+
+  int tm, tn;
+  if (!tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn)) return;
+  const int64_t m0 = (int64_t)tm * T::BM, n0 = (int64_t)tn * T::BN;
+  Loader<T> loader(p, lds, m0, n0, wave, lane);
+
+  const int64_t m = m0 + wm * 16 * MT + c * MT, n = n0 + wn * 16 * NT + g * 4 * NT;
+  const int64_t sa_at = min(m, p.sa_pitch - 8);       // rows past the end take scales of the last ones
+  const int64_t sb_at = min(n0 + wn * 16 * NT, p.n - 1) / kBlockK * p.kb;
+  Scales<POW2> sa;
+  float sb_f = 0.f;
+  uint32_t sb_b = 0;
+  auto scales = [&](int kb) {
+    sa.load(p.sa, kb * p.sa_pitch + sa_at);
+    if constexpr (POW2) sb_b = ((const uint8_t*)p.sb)[sb_at + kb];
+    else sb_f = ((const float*)p.sb)[sb_at + kb];
+  };
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const uint8_t* la = lds + (wm * 16 * MT + c * MT) * kBlockK;
+  const uint8_t* lb = lds + T::BM * kBlockK + (wn * 16 * NT + (c >> 2) * 4 * NT + (c & 3)) * kBlockK;
+  const int piece0 = (g ^ (c & 7)) * 16, piece1 = piece0 ^ 64;
+
+  loader.fetch(0, 0);
+  scales(0);
+  for (int kb = 0; kb < p.kb; ++kb) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    sa.arrived();
+    Scales<POW2> now = sa;
+    const float wf = sb_f;
+    const uint32_t wb = sb_b;
+    if (kb + 1 < p.kb) {
+      scales(kb + 1);
+      loader.fetch(kb + 1, (kb + 1) & 1);
+    }
+    const int buf = (kb & 1) * T::kBytes;
+    i32x8 w[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const i32x4 x = *(const i32x4*)(lb + buf + j * 4 * kBlockK + piece0);
+      const i32x4 y = *(const i32x4*)(lb + buf + j * 4 * kBlockK + piece1);
+      w[j] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    auto row = [&](auto I) {
+      constexpr int i = decltype(I)::value;
+      const i32x4 x = *(const i32x4*)(la + buf + i * kBlockK + piece0);
+      const i32x4 y = *(const i32x4*)(la + buf + i * kBlockK + piece1);
+      const i32x8 v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if constexpr (POW2) {
+          acc[i][j] = mfma_scaled<i & 3>(w[j], v, acc[i][j], wb, now.b[i >> 2]);
+        } else {
+          const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+          const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[j], v, zero, 0, 0, 0, 0, 0, 0);
+          const float s = now.f[i] * wf;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[r], s, acc[i][j][r]);
+        }
+      }
+    };
+    each<MT>(row);
+  }
+
+  store_tile<MT, NT, O>(p, acc, m, n);
+}
+
+// The same tile for e8m0 scales with four waves of 128 x 128, one to a SIMD: the matrix instruction
+// applies the scales, so the sums never leave the accumulation registers, and half as many bytes leave LDS as
+// with eight waves of 128 x 64 (128 KB a step instead of 192 KB, at 128 B a cycle and 2048 cycles of products).
+//
+// A step is four quarters of 16 products: rows x0, x1 (four 16-row pieces each) times columns w0, w1.
+// Each quarter loads from LDS what a later one needs, into what has been left:
+//   x0 w0 (load w1)   x0 w1 (load x1)  | x1 w1 (load next x0)   x1 w0 (load next w0, piece by piece)
+// At "|" every wave has read the step's tile, so its half of LDS is filled again, for the step after
+// the next: a load has a whole step to arrive. The last steps load their own tile once more, which nobody reads.
+template <typename O>
+__global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int tiles_n) {
+  using T = Tile<8, 8, 2, 2>;
+  constexpr int MT = 8, NT = 8;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * T::kBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4, wm = wave / T::WN, wn = wave % T::WN;
+  int tm, tn;
+  if (!tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn)) return;
+  const int64_t m0 = (int64_t)tm * T::BM, n0 = (int64_t)tn * T::BN;
+  Loader<T> loader(p, lds, m0, n0, wave, lane);
+
+  const int64_t m = m0 + wm * 16 * MT + c * MT, n = n0 + wn * 16 * NT + g * 4 * NT;
+  const uint8_t* sa = (const uint8_t*)p.sa + min(m, p.sa_pitch - 8);
+  const uint8_t* sb = (const uint8_t*)p.sb + min(n0 + wn * 16 * NT, p.n - 1) / kBlockK * p.kb;
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int piece = (g ^ (c & 7)) * 16;
+  const uint8_t* la = lds + (wm * 16 * MT + c * MT) * kBlockK;
+  const uint8_t* lb = lds + T::BM * kBlockK + (wn * 16 * NT + (c >> 2) * 4 * NT + (c & 3)) * kBlockK;
+  i32x4 x[8][2], w[8][2];            // [piece][k half]
+  auto read_x = [&](int buf, int k, int h) { x[k][h] = *(const i32x4*)(la + buf + k * kBlockK + (h ? piece ^ 64 : piece)); };
+  auto read_w = [&](int buf, int k, int h) { w[k][h] = *(const i32x4*)(lb + buf + k * 4 * kBlockK + (h ? piece ^ 64 : piece)); };
+
+  Scales<true> next, now;
+  uint32_t next_b, now_b;
+  loader.fetch(0, 0);
+  next.load(sa, 0);
+  next_b = sb[0];
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  next.arrived();
+  asm volatile("" : "+v"(next_b));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  loader.fetch(min(1, p.kb - 1), 1);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    read_x(0, k, 0), read_x(0, k, 1);
+    read_w(0, k, 0), read_w(0, k, 1);
+  }
+
+#pragma unroll 1
+  for (int kb = 0; kb < p.kb; ++kb) {
+    const int buf = (kb & 1) * T::kBytes, ahead = T::kBytes - buf;
+    const int kb1 = min(kb + 1, p.kb - 1), kb2 = min(kb + 2, p.kb - 1);
+    now = next;
+    now_b = next_b;
+    // product number `at` of a quarter, one column piece after the other
+    auto quarter = [&](auto Rows, auto Cols, auto between) {
+      constexpr int r = decltype(Rows)::value, q = decltype(Cols)::value;
+      auto one = [&](auto At) {
+        constexpr int at = decltype(At)::value, i = r * 4 + at % 4, j = q * 4 + at / 4;
+        acc[i][j] = mfma_scaled<i & 3>(join(w[j]), join(x[i]), acc[i][j], now_b, now.b[r]);
+        between(at);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      each<16>(one);
+    };
+    quarter(Index<0>{}, Index<0>{}, [&](int at) {
+      if (at < 8) read_w(buf, 4 + at / 2, at % 2);
+      if (at == 8) next.load(sa, kb1 * p.sa_pitch);
+      if (at == 9) next_b = sb[kb1];
+    });
+    quarter(Index<0>{}, Index<1>{}, [&](int at) {
+      if (at < 8) read_x(buf, 4 + at / 2, at % 2);
+    });
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    next.arrived();
+    asm volatile("" : "+v"(next_b));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    quarter(Index<1>{}, Index<1>{}, [&](int at) {
+      if (at < 8) read_x(ahead, at / 2, at % 2);
+      loader.one(at, kb2, kb & 1);
+    });
+    quarter(Index<1>{}, Index<0>{}, [&](int at) {
+      if (at % 4 == 3) read_w(ahead, at / 4, 0), read_w(ahead, at / 4, 1);
+    });
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing may reach LDS after the workgroup's end
+  store_tile<MT, NT, O>(p, acc, m, n);
+}
+
 template <typename T, typename O>
 int run_tile(const MatArgs& p, bool pow2, hipStream_t s) {
   const int64_t tm = (p.m + T::BM - 1) / T::BM, tn = (p.n + T::BN - 1) / T::BN, total = tm * tn;
@@ -316,6 +424,14 @@ int run_tile(const MatArgs& p, bool pow2, hipStream_t s) {
 using Big = Tile<8, 4, 2, 4>;
 
 template <typename O>
+int run_quarters(const MatArgs& p, hipStream_t s) {
+  const int64_t tm = (p.m + 255) / 256, tn = (p.n + 255) / 256, total = tm * tn;
+  if (total > (1 << 30)) return -1;
+  k_quarters<O><<<(unsigned)((total + 7) / 8 * 8), 256, 0, s>>>(p, (int)tm, (int)tn);
+  return (int)hipGetLastError();
+}
+
+template <typename O>
 int run_simple(const MatArgs& p, bool pow2, hipStream_t s) {
   const int64_t gx = (p.n + 63) / 64, gy = (p.m + 15) / 16;
   if (gx > 0x7FFFFFFF || gy > 65535) return -1;
@@ -327,7 +443,7 @@ int run_simple(const MatArgs& p, bool pow2, hipStream_t s) {
 
 template <typename O>
 int run(const MatArgs& p, bool pow2, hipStream_t s) {
-  if (p.m > 64) return run_tile<Big, O>(p, pow2, s);
+  if (p.m > 64) return pow2 ? run_quarters<O>(p, s) : run_tile<Big, O>(p, pow2, s);
   return run_simple<O>(p, pow2, s);
 }
 
@@ -338,16 +454,17 @@ using namespace yoda_fp8;
 
 extern "C" {
 
-// kb: blocks along K. pitch: elements between rows of out. Returns 0, a hipError, or -1 for
+// kb: blocks along K. pitch: elements between rows of out. sa_pitch: scales between a's blocks along K,
+// a multiple of 8, the scales 16-byte aligned. Returns 0, a hipError, or -1 for
 // arguments out of range.
 int yoda_fp8_matmul(int device, void* stream, int out_type, int pow2, const void* a, const void* sa, const void* b,
-                    const void* sb, const void* bias, void* out, int64_t m, int64_t n, int kb, int64_t pitch) {
-  if ((out_type != kBf16 && out_type != kFp16) || m < 0 || n < 0 || kb < 1 || kb > 65535 || pitch < n) return -1;
+                    const void* sb, const void* bias, void* out, int64_t m, int64_t n, int kb, int64_t pitch, int64_t sa_pitch) {
+  if ((out_type != kBf16 && out_type != kFp16) || m < 0 || n < 0 || kb < 1 || kb > 65535 || pitch < n || sa_pitch < m || sa_pitch % 8) return -1;
   if (m == 0 || n == 0) return 0;
   if (!a || !sa || !b || !sb || !out) return -1;
   DeviceScope on(device);
   if (on.err != hipSuccess) return (int)on.err;
-  const MatArgs p = {(const uint8_t*)a, (const uint8_t*)b, sa, sb, bias, out, m, n, pitch, kb};
+  const MatArgs p = {(const uint8_t*)a, (const uint8_t*)b, sa, sb, bias, out, m, n, pitch, sa_pitch, kb};
   const hipStream_t s = (hipStream_t)stream;
   if (out_type == kFp16) return run<__half>(p, pow2, s);
   return run<__hip_bfloat16>(p, pow2, s);

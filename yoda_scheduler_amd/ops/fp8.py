@@ -48,12 +48,18 @@ def blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
+def _row_scales(rows: int, kb: int, dtype: torch.dtype, device, zeros: bool = False) -> torch.Tensor:
+    """[rows, kb] scales of 1 x 128 blocks: kb runs of ``rows``, a multiple of 8 apart."""
+    make = torch.zeros if zeros else torch.empty
+    return make((kb, -(-rows // 8) * 8), dtype=dtype, device=device)[:, :rows].t()
+
+
 class BlockMatrix:
     """``rows`` × ``cols`` values in e4m3 with a scale for each block.
 
     ``data``    [rows, 128 · blocks(cols)] e4m3, contiguous; the columns from ``cols`` on are zero
     ``scales``  [blocks of rows, blocks of columns], float32 or e8m0. For ``block_rows`` 1 they lie
-                block by block (``scales.t()`` is contiguous), for 128 row by row.
+                block by block, each block's rows padded to a multiple of 8, for 128 row by row.
 
     The constructor takes values that exist already (a checkpoint's): unpadded ones and scales in
     the other order are laid out once, here. Padded ones must hold zeros from ``cols`` on.
@@ -88,8 +94,9 @@ class BlockMatrix:
         if values.data_ptr() % 16:
             values = values.clone()
         if block_rows == 1:
-            if not scales.t().is_contiguous():
-                scales = scales.t().contiguous().t()
+            pitch = -(-rows // 8) * 8
+            if scales.stride() != (1, pitch) or scales.data_ptr() % 16:
+                scales = _row_scales(rows, kb, scales.dtype, scales.device, zeros=True).copy_(scales)
         elif not scales.is_contiguous():
             scales = scales.contiguous()
         self.data, self.scales, self.rows, self.cols, self.block_rows = values, scales, rows, cols, block_rows
@@ -100,7 +107,7 @@ class BlockMatrix:
         kb = blocks(cols)
         m.data = torch.empty((rows, kb * BLOCK), dtype=E4M3, device=device)
         if block_rows == 1:
-            m.scales = torch.empty((kb, rows), dtype=scale_dtype, device=device).t()
+            m.scales = _row_scales(rows, kb, scale_dtype, device)
         else:
             m.scales = torch.empty((blocks(rows), kb), dtype=scale_dtype, device=device)
         m.rows, m.cols, m.block_rows = rows, cols, block_rows
@@ -245,5 +252,5 @@ def matmul(a: BlockMatrix, b: BlockMatrix, out_dtype: torch.dtype = torch.bfloat
     _ok(_lib()[2](device.index, _stream(device), _OUT[out_dtype], a.scales.dtype is E8M0, a.data.data_ptr(),
                   a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(),
                   None if bias is None else bias.data_ptr(), out.data_ptr(), m, n, blocks(a.cols),
-                  max(out.stride(0), n)), "fp8 matmul")
+                  max(out.stride(0), n), -(-m // 8) * 8), "fp8 matmul")
     return out

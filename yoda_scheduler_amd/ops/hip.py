@@ -49,7 +49,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "yoda_fp8_quantize": [c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
                               c_int],
         "yoda_fp8_matmul": [c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                            c_int64, c_int64, c_int, c_int64],
+                            c_int64, c_int64, c_int, c_int64, c_int64],
     }
     for name, args in sigs.items():
         f = getattr(lib, name, None)
