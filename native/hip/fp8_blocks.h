@@ -41,6 +41,7 @@ struct DeviceScope {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float to_f32(uint16_t v, __hip_bfloat16*) { return __uint_as_float((uint32_t)v << 16); }
 __device__ __forceinline__ float to_f32(uint16_t v, __half*) { return __half2float(__ushort_as_half(v)); }
@@ -71,5 +72,34 @@ __device__ __forceinline__ typename Bits<T>::type store_bits(float v) {
     return __builtin_bit_cast(uint16_t, b);
   }
 }
+
+// Two float32 to two neighbours of a 16-bit type, to nearest, ties to even.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (__is_same(T, __half)) {
+    return (uint32_t)store_bits<__half>(a) | (uint32_t)store_bits<__half>(b) << 16;
+  } else {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  }
+}
+
+// 16 bytes at any element of 2 or 4 bytes: one access, whatever the row's pitch. (A packed struct of
+// elements would be taken apart into one access an element.)
+typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+template <int SIZE>
+struct Wide {
+  using type = u32x4_at2;
+  static __device__ __forceinline__ u32x4 load(const void* p) { return *(const type*)p; }
+  static __device__ __forceinline__ void store(void* p, u32x4 v) { *(type*)p = v; }
+};
+template <>
+struct Wide<4> {
+  using type = u32x4_at4;
+  static __device__ __forceinline__ u32x4 load(const void* p) { return *(const type*)p; }
+  static __device__ __forceinline__ void store(void* p, u32x4 v) { *(type*)p = v; }
+};
 
 }  // namespace yoda_fp8

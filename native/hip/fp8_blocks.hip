@@ -81,17 +81,23 @@ __device__ __forceinline__ uint2 to_e4m3(const float (&v)[kWidth], float inv) {
 }
 
 // Eight neighbours of a row from column c on; zeros from column `cols` on. The rows of a caller's
-// matrix start at any element, so the wide load assumes no more than an element's alignment.
+// matrix start at any element, so the wide access assumes no more than an element's alignment.
 template <typename T>
 __device__ __forceinline__ void load8(const T* row, int c, int cols, float (&v)[kWidth]) {
   using B = typename Bits<T>::type;
-  struct __attribute__((packed, aligned(sizeof(B)))) Eight {
-    B b[kWidth];
-  };
   if (c + kWidth <= cols) {
-    const Eight e = *(const Eight*)(row + c);
+    const u32x4 a = Wide<sizeof(T)>::load(row + c);
+    if constexpr (sizeof(T) == 4) {
+      const u32x4 b = Wide<4>::load(row + c + 4);
 #pragma unroll
-    for (int i = 0; i < kWidth; ++i) v[i] = load_f32<T>(e.b[i]);
+      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(a[i]), v[4 + i] = __uint_as_float(b[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = load_f32<T>((uint16_t)(a[i] & 0xFFFF));
+        v[2 * i + 1] = load_f32<T>((uint16_t)(a[i] >> 16));
+      }
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < kWidth; ++i) v[i] = c + i < cols ? load_f32<T>(((const B*)row)[c + i]) : 0.f;
@@ -101,18 +107,22 @@ __device__ __forceinline__ void load8(const T* row, int c, int cols, float (&v)[
 template <typename T>
 __device__ __forceinline__ void store8(T* row, int c, int cols, const float (&v)[kWidth]) {
   using B = typename Bits<T>::type;
-  struct __attribute__((packed, aligned(sizeof(B)))) Eight {
-    B b[kWidth];
-  };
-  Eight e;
-#pragma unroll
-  for (int i = 0; i < kWidth; ++i) e.b[i] = store_bits<T>(v[i]);
   if (c + kWidth <= cols) {
-    *(Eight*)(row + c) = e;
+    u32x4 a;
+    if constexpr (sizeof(T) == 4) {
+      u32x4 b;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = __float_as_uint(v[i]), b[i] = __float_as_uint(v[4 + i]);
+      Wide<4>::store(row + c + 4, b);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    }
+    Wide<sizeof(T)>::store(row + c, a);
   } else {
 #pragma unroll
     for (int i = 0; i < kWidth; ++i)
-      if (c + i < cols) ((B*)row)[c + i] = e.b[i];
+      if (c + i < cols) ((B*)row)[c + i] = store_bits<T>(v[i]);
   }
 }
 

@@ -98,14 +98,20 @@ struct Tile {
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "whole loads for every wave");
 };
 
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-
-// Lane l's 16 bytes at base + voff + soff go to LDS at lds + 16 l.
+// Lane l's BYTES at base + voff + soff go to LDS at lds + BYTES * l. (m0 is the compiler's to set before its
+// own uses of it, and it makes none here.)
+template <int BYTES>
 __device__ __forceinline__ void load_lds(u32x4 rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
-               : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
-               : "memory");
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
+                 : "memory");
 }
 
 __device__ __forceinline__ u32x4 buffer_of(const void* base) {
@@ -197,9 +203,9 @@ struct Loader {
   __device__ __forceinline__ void one(int i, int kb, int buf) {
     const uint32_t to = base + buf * T::kBytes;
     if (i < T::kLoadsA)
-      load_lds(ra, va[i], kb * kBlockK, to + (wave + i * T::kWaves) * 1024);
+      load_lds<16>(ra, va[i], kb * kBlockK, to + (wave + i * T::kWaves) * 1024);
     else
-      load_lds(rb, vb[i - T::kLoadsA], kb * kBlockK, to + T::BM * kBlockK + (wave + (i - T::kLoadsA) * T::kWaves) * 1024);
+      load_lds<16>(rb, vb[i - T::kLoadsA], kb * kBlockK, to + T::BM * kBlockK + (wave + (i - T::kLoadsA) * T::kWaves) * 1024);
   }
   __device__ __forceinline__ void fetch(int kb, int buf) {
 #pragma unroll
@@ -207,28 +213,45 @@ struct Loader {
   }
 };
 
+// A lane's MT rows from m on, 4 * NT neighbouring columns from n on.
 template <int MT, int NT, typename O>
 __device__ __forceinline__ void store_tile(const MatArgs& p, const f32x4 (&acc)[MT][NT], int64_t m, int64_t n) {
   using B = typename Bits<O>::type;
-  float bias[NT * 4];
+  f32x4 bias[NT];
 #pragma unroll
-  for (int k = 0; k < NT * 4; ++k) bias[k] = p.bias && n + k < p.n ? load_f32<O>(((const B*)p.bias)[n + k]) : 0.f;
-  struct __attribute__((packed, aligned(sizeof(B)))) Out { B b[NT * 4]; };
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    if (m + i >= p.m) break;
-    Out o;
+  for (int j = 0; j < NT; ++j) bias[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (p.bias) {
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o.b[4 * j + r] = store_bits<O>(acc[i][j][r] + bias[4 * j + r]);
-    B* to = (B*)p.out + (m + i) * p.pitch + n;
-    if (n + NT * 4 <= p.n) {
-      *(Out*)to = o;
-    } else {
+      for (int r = 0; r < 4; ++r) bias[j][r] = load_f32<O>(((const B*)p.bias)[min(n + 4 * j + r, p.n - 1)]);
+  }
+  if (m >= p.m || n >= p.n) return;
+  B* out = (B*)p.out + m * p.pitch + n;
+  const int rows = (int)min((int64_t)MT, p.m - m);
+  if (n + 4 * NT <= p.n) {
 #pragma unroll
-      for (int k = 0; k < NT * 4; ++k)
-        if (n + k < p.n) to[k] = o.b[k];
+    for (int i = 0; i < MT; ++i) {
+      if (i >= rows) break;
+#pragma unroll
+      for (int j = 0; j < NT; j += 2) {
+        const f32x4 u = acc[i][j] + bias[j], v = acc[i][j + 1] + bias[j + 1];
+        Wide<sizeof(B)>::store(out + 4 * j, u32x4{pack2<O>(u[0], u[1]), pack2<O>(u[2], u[3]), pack2<O>(v[0], v[1]),
+                                                  pack2<O>(v[2], v[3])});
+      }
+      out += p.pitch;
+    }
+  } else {
+    const int cols = (int)(p.n - n);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if (i >= rows) break;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (4 * j + r < cols) out[4 * j + r] = store_bits<O>(acc[i][j][r] + bias[j][r]);
+      out += p.pitch;
     }
   }
 }
@@ -314,101 +337,173 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 2 : 1) void k_til
   store_tile<MT, NT, O>(p, acc, m, n);
 }
 
-// The same tile for e8m0 scales with four waves of 128 x 128, one to a SIMD: the matrix instruction
-// applies the scales, so the sums never leave the accumulation registers, and half as many bytes leave LDS as
-// with eight waves of 128 x 64 (128 KB a step instead of 192 KB, at 128 B a cycle and 2048 cycles of products).
+// 256 x 256 for e8m0 scales with four waves of 128 x 128, one to a SIMD: the matrix instruction applies
+// the scales, so the sums never leave the accumulation registers, and fewer bytes leave LDS than with
+// eight waves of 128 x 64 (128 KB a step instead of 192 KB, at 128 B a cycle and 2048 cycles of products).
 //
-// A step is four quarters of 16 products: rows x0, x1 (four 16-row pieces each) times columns w0, w1.
-// Each quarter loads from LDS what a later one needs, into what has been left:
-//   x0 w0 (load w1)   x0 w1 (load x1)  | x1 w1 (load next x0)   x1 w0 (load next w0, piece by piece)
-// At "|" every wave has read the step's tile, so its half of LDS is filled again, for the step after
-// the next: a load has a whole step to arrive. The last steps load their own tile once more, which nobody reads.
-template <typename O>
-__global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int tiles_n) {
-  using T = Tile<8, 8, 2, 2>;
-  constexpr int MT = 8, NT = 8;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * T::kBytes];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4, wm = wave / T::WN, wn = wave % T::WN;
-  int tm, tn;
-  if (!tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn)) return;
-  const int64_t m0 = (int64_t)tm * T::BM, n0 = (int64_t)tn * T::BN;
-  Loader<T> loader(p, lds, m0, n0, wave, lane);
+// A step is four quarters of 16 products: rows x0, x1 (four pieces of 16 each) times columns w0, w1.
+// Each quarter reads from LDS what a later one needs and loads 16 KB of the step after the next
+// into what every wave has read:
+//            products   reads                       loads
+//   Q0(k)    x0 w0      w1(k)                       x0(k+2)
+//   Q1(k)    x0 w1      x1(k)                       w0(k+2)
+//   Q2(k)    x1 w1      x0(k+1)                     w1(k+2)
+//   Q3(k)    x1 w0      w0(k+1), piece by piece     x1(k+2), rows' scales(k+3)
+// A load has six quarters (3072 cycles) to arrive; every wave counts its own loads (4, 4, 4 and 5 a quarter)
+// and waits for those that the quarter reads, and the barrier joins the waits of all four. What a
+// quarter loads into was read a step before (x0: waited for by count at Q0; the others: their
+// products have been issued). The last steps load their last tile again, which nobody reads.
+struct Quarters {
+  static constexpr int BM = 256, BN = 256, kThreads = 256;
+  static constexpr int kPart = 128 * kBlockK;                     // x0, x1, w0 or w1 of one step: 16 KB
+  static constexpr int kStep = 4 * kPart, kScales = 2 * kStep;    // then 4 steps x 4 waves x 256 scales
+  static constexpr int kLds = kScales + 4 * 4 * 256;
+};
 
-  const int64_t m = m0 + wm * 16 * MT + c * MT, n = n0 + wn * 16 * NT + g * 4 * NT;
-  const uint8_t* sa = (const uint8_t*)p.sa + min(m, p.sa_pitch - 8);
-  const uint8_t* sb = (const uint8_t*)p.sb + min(n0 + wn * 16 * NT, p.n - 1) / kBlockK * p.kb;
-
-  f32x4 acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const int piece = (g ^ (c & 7)) * 16;
-  const uint8_t* la = lds + (wm * 16 * MT + c * MT) * kBlockK;
-  const uint8_t* lb = lds + T::BM * kBlockK + (wn * 16 * NT + (c >> 2) * 4 * NT + (c & 3)) * kBlockK;
-  i32x4 x[8][2], w[8][2];            // [piece][k half]
-  auto read_x = [&](int buf, int k, int h) { x[k][h] = *(const i32x4*)(la + buf + k * kBlockK + (h ? piece ^ 64 : piece)); };
-  auto read_w = [&](int buf, int k, int h) { w[k][h] = *(const i32x4*)(lb + buf + k * 4 * kBlockK + (h ? piece ^ 64 : piece)); };
-
-  Scales<true> next, now;
-  uint32_t next_b, now_b;
-  loader.fetch(0, 0);
-  next.load(sa, 0);
-  next_b = sb[0];
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  next.arrived();
-  asm volatile("" : "+v"(next_b));
+// wait for all but `left` of the wave's loads, then for the other waves
+template <int LEFT>
+__device__ __forceinline__ void meet() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  loader.fetch(min(1, p.kb - 1), 1);
+}
+
+template <typename O>
+__global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int tiles_n) {
+  using Q = Quarters;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Q::kLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
+  int tm, tn;
+  if (!tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn)) return;
+  const int64_t m0 = (int64_t)tm * Q::BM, n0 = (int64_t)tn * Q::BN, kp = (int64_t)p.kb * kBlockK;
+  const int64_t m = m0 + wm * 128 + c * 8, n = n0 + wn * 128 + g * 32;
+  const int last = p.kb - 1;
+
+  // LDS rows of a part: x: 64 * wm + 4 * c + i for row 128 * wm + 8 * c + 4 * part + i,
+  // w: 64 * wn + 16 * (c / 4) + 4 * j + c % 4 for column 128 * wn + 32 * (c / 4) + 16 * part + 4 * j + c % 4
+  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  const u32x4 rx = buffer_of(p.a + m0 * kp), rw = buffer_of(p.b + n0 * kp);
+  uint32_t vx[8], vw[8];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    read_x(0, k, 0), read_x(0, k, 1);
-    read_w(0, k, 0), read_w(0, k, 1);
+  for (int part = 0; part < 2; ++part)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = (wave + 4 * i) * 8 + lane / 8;              // of the part, in LDS
+      const int64_t xm = (row >> 6) * 128 + (row >> 2 & 15) * 8 + part * 4 + (row & 3);
+      const int64_t wc = (row >> 6) * 128 + (row >> 4 & 3) * 32 + part * 16 + (row & 15);
+      const int kx = row >> 2 & 7, kw = (row & 3) | (row >> 4 & 1) << 2;
+      vx[part * 4 + i] = (uint32_t)(min(xm, p.m - 1 - m0) * kp + ((lane & 7) ^ kx) * 16);
+      vw[part * 4 + i] = (uint32_t)(min(wc, p.n - 1 - n0) * kp + ((lane & 7) ^ kw) * 16);
+    }
+  const uint32_t vs = (uint32_t)min((int64_t)lane * 4, p.sa_pitch - 4 - m0);
+  auto load_x = [&](int part, int i, int k) {
+    load_lds<16>(rx, vx[part * 4 + i], min(k, last) * kBlockK,
+                 base + (k & 1) * Q::kStep + part * Q::kPart + (wave + 4 * i) * 1024);
+  };
+  auto load_w = [&](int part, int i, int k) {
+    load_lds<16>(rw, vw[part * 4 + i], min(k, last) * kBlockK,
+                 base + (k & 1) * Q::kStep + (2 + part) * Q::kPart + (wave + 4 * i) * 1024);
+  };
+  auto load_s = [&](int k) {
+    const u32x4 rs = buffer_of((const uint8_t*)p.sa + m0 + min(k, last) * p.sa_pitch);
+    load_lds<4>(rs, vs, 0, base + Q::kScales + ((k & 3) * 4 + wave) * 256);
+  };
+
+  const int piece = (g ^ (c & 7)) * 16;
+  const uint8_t* lx = lds + (wm * 64 + c * 4) * kBlockK;
+  const uint8_t* lw = lds + 2 * Q::kPart + (wn * 64 + (c >> 2) * 16 + (c & 3)) * kBlockK;
+  const uint8_t* ls = lds + Q::kScales + wave * 256 + wm * 128 + c * 8;
+  i32x4 x[8][2], w[8][2];            // [piece][half of its 32 bytes]
+  auto read_x = [&](int k, int i, int h) {
+    x[i][h] = *(const i32x4*)(lx + (k & 1) * Q::kStep + (i >> 2) * Q::kPart + (i & 3) * kBlockK + (h ? piece ^ 64 : piece));
+  };
+  auto read_w = [&](int k, int j, int h) {
+    w[j][h] = *(const i32x4*)(lw + (k & 1) * Q::kStep + (j >> 2) * Q::kPart + (j & 3) * 4 * kBlockK + (h ? piece ^ 64 : piece));
+  };
+
+  // the columns' scales of 256 steps: four in each lane
+  const uint8_t* sb = (const uint8_t*)p.sb + min(n0 + wn * 128, p.n - 1) / kBlockK * p.kb;
+  auto column_scales = [&](int k) {
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v |= (uint32_t)sb[min(k + lane * 4 + i, last)] << (8 * i);
+    return v;
+  };
+  uint32_t sbs = column_scales(0);
+  asm volatile("" : "+v"(sbs));
+
+  f32x4 acc[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  auto four = [&](auto load) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load(i);
+  };
+  load_s(0);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    four([&](int i) { load_x(0, i, k); });
+    four([&](int i) { load_w(0, i, k); });
+    four([&](int i) { load_w(1, i, k); });
+    load_s(k + 1);
+    four([&](int i) { load_x(1, i, k); });
   }
+  meet<26>();
+  uint2 next = *(const uint2*)ls, now;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) read_x(0, i, 0), read_x(0, i, 1);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) read_w(0, j, 0), read_w(0, j, 1);
 
 #pragma unroll 1
-  for (int kb = 0; kb < p.kb; ++kb) {
-    const int buf = (kb & 1) * T::kBytes, ahead = T::kBytes - buf;
-    const int kb1 = min(kb + 1, p.kb - 1), kb2 = min(kb + 2, p.kb - 1);
-    now = next;
-    now_b = next_b;
-    // product number `at` of a quarter, one column piece after the other
+  for (int k = 0; k < p.kb; ++k) {
+    if ((k & 255) == 0 && k) {
+      sbs = column_scales(k);
+      asm volatile("" : "+v"(sbs));
+    }
+    // product number `at` of a quarter, one piece of columns after the other
     auto quarter = [&](auto Rows, auto Cols, auto between) {
       constexpr int r = decltype(Rows)::value, q = decltype(Cols)::value;
+      const uint32_t ws = __builtin_amdgcn_readlane(sbs, k >> 2 & 63) >> (8 * (k & 3));
       auto one = [&](auto At) {
         constexpr int at = decltype(At)::value, i = r * 4 + at % 4, j = q * 4 + at / 4;
-        acc[i][j] = mfma_scaled<i & 3>(join(w[j]), join(x[i]), acc[i][j], now_b, now.b[r]);
+        acc[i][j] = mfma_scaled<i & 3>(join(w[j]), join(x[i]), acc[i][j], ws, r ? now.y : now.x);
         between(at);
         __builtin_amdgcn_sched_barrier(0);
       };
       each<16>(one);
     };
+    asm volatile("s_waitcnt lgkmcnt(8)" ::: "memory");            // x0(k) and the scales are in registers
+    meet<22>();
+    now = next;
     quarter(Index<0>{}, Index<0>{}, [&](int at) {
-      if (at < 8) read_w(buf, 4 + at / 2, at % 2);
-      if (at == 8) next.load(sa, kb1 * p.sa_pitch);
-      if (at == 9) next_b = sb[kb1];
+      if (at < 8) read_w(k, 4 + at / 2, at % 2);
+      if (at % 4 == 2) load_x(0, at / 4, k + 2);
     });
+    meet<21>();
     quarter(Index<0>{}, Index<1>{}, [&](int at) {
-      if (at < 8) read_x(buf, 4 + at / 2, at % 2);
+      if (at < 8) read_x(k, 4 + at / 2, at % 2);
+      if (at % 4 == 2) load_w(0, at / 4, k + 2);
     });
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    next.arrived();
-    asm volatile("" : "+v"(next_b));
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    meet<21>();
     quarter(Index<1>{}, Index<1>{}, [&](int at) {
-      if (at < 8) read_x(ahead, at / 2, at % 2);
-      loader.one(at, kb2, kb & 1);
+      if (at < 8) read_x(k + 1, at / 2, at % 2);
+      if (at % 4 == 2) load_w(1, at / 4, k + 2);
     });
+    meet<21>();
+    next = *(const uint2*)(ls + (k + 1 & 3) * 1024);
     quarter(Index<1>{}, Index<0>{}, [&](int at) {
-      if (at % 4 == 3) read_w(ahead, at / 4, 0), read_w(ahead, at / 4, 1);
+      if (at == 0) load_s(k + 3);
+      if (at % 4 == 2) load_x(1, at / 4, k + 2);
+      if (at % 4 == 3) read_w(k + 1, at / 4, 0), read_w(k + 1, at / 4, 1);
     });
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing may reach LDS after the workgroup's end
-  store_tile<MT, NT, O>(p, acc, m, n);
+  store_tile<8, 8, O>(p, acc, m, n);
 }
 
 template <typename T, typename O>
