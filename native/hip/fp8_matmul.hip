@@ -79,15 +79,18 @@ __global__ __launch_bounds__(256) void k_simple(MatArgs p) {
 // ---------------------------------------------------------------- tiles through LDS
 //
 // One workgroup a tile of BM x BN, 128 of K a step: each wave holds 16*MT rows m times 16*NT columns
-// n of sums. Rows and columns are dealt to the lanes so that what belongs to a lane lies together:
-// lane (c, g) = (lane % 16, lane / 16) has the rows m = c*MT + i of its wave (i < MT: one load brings
-// its scales) and the columns n = g*4*NT + 4*j + r (j < NT, r < 4: it stores 4*NT neighbours).
+// n of sums. Lane (c, g) = (lane % 16, lane / 16) has the rows m = c*MT + i of its wave (i < MT), so that one
+// load brings its scales, and of column piece j the four columns that make, over two pieces and the
+// four g, 32 neighbours: a store writes 64 bytes of a row, 16 from each g.
 //
-// Both tiles lie in LDS as rows of 128 bytes, their eight 16-byte pieces exchanged by
-// piece ^= key(row), key = the low three bits of the c that reads the row, so that eight lanes which
-// read a piece of eight rows at once meet eight different bank groups. The loads go from memory into LDS
-// directly: lane l of a load fills piece l % 8 of row l / 8, and takes the piece of memory that
-// belongs there.
+// Both tiles lie in LDS as rows of 128 bytes, 16 rows a piece in the order of the c that reads them.
+// The eight 16-byte parts of a row are exchanged by part ^= (row / 2) % 8, so that sixteen lanes that are
+// served at once meet sixteen different parts of 256 bytes (64 banks). The loads go from memory into LDS directly: lane
+// l of a load fills part l % 8 of row l / 8, and takes the part of memory that belongs there.
+__host__ __device__ __forceinline__ constexpr int column_of(int piece, int c) {
+  return (piece >> 1) * 32 + (c >> 2) * 8 + (piece & 1) * 4 + (c & 3);
+}
+
 template <int MT_, int NT_, int WM_, int WN_>
 struct Tile {
   static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_;
@@ -188,15 +191,15 @@ struct Loader {
     rb = buffer_of(p.b + n0 * kp);
 #pragma unroll
     for (int i = 0; i < T::kLoadsA; ++i) {
-      const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = row / T::MT & 7;
-      const int64_t in = m0 + row < p.m ? row : p.m - 1 - m0;
-      va[i] = (uint32_t)(in * kp + ((lane & 7) ^ key) * 16);
+      const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = row >> 1 & 7, piece = row >> 4;
+      const int64_t in = piece / T::MT * 16 * T::MT + (row & 15) * T::MT + piece % T::MT;
+      va[i] = (uint32_t)(min(in, p.m - 1 - m0) * kp + ((lane & 7) ^ key) * 16);
     }
 #pragma unroll
     for (int i = 0; i < T::kLoadsB; ++i) {
-      const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = (row & 3) | (row / (4 * T::NT) & 1) << 2;
-      const int64_t in = n0 + row < p.n ? row : p.n - 1 - n0;
-      vb[i] = (uint32_t)(in * kp + ((lane & 7) ^ key) * 16);
+      const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = row >> 1 & 7, piece = row >> 4;
+      const int64_t in = piece / T::NT * 16 * T::NT + column_of(piece % T::NT, row & 15);
+      vb[i] = (uint32_t)(min(in, p.n - 1 - n0) * kp + ((lane & 7) ^ key) * 16);
     }
   }
   // load i of the step's kLoadsA + kLoadsB
@@ -213,45 +216,42 @@ struct Loader {
   }
 };
 
-// A lane's MT rows from m on, 4 * NT neighbouring columns from n on.
+// A lane's MT rows from m on; n: the wave's first column.
 template <int MT, int NT, typename O>
-__device__ __forceinline__ void store_tile(const MatArgs& p, const f32x4 (&acc)[MT][NT], int64_t m, int64_t n) {
+__device__ __forceinline__ void store_tile(const MatArgs& p, const f32x4 (&acc)[MT][NT], int64_t m, int64_t n, int g) {
   using B = typename Bits<O>::type;
-  f32x4 bias[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) bias[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (p.bias) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) bias[j][r] = load_f32<O>(((const B*)p.bias)[min(n + 4 * j + r, p.n - 1)]);
-  }
-  if (m >= p.m || n >= p.n) return;
-  B* out = (B*)p.out + m * p.pitch + n;
+  n += g * 8;                           // of pieces 2j and 2j + 1: columns 32 j .. 32 j + 7 from here
+  if (m >= p.m) return;
   const int rows = (int)min((int64_t)MT, p.m - m);
-  if (n + 4 * NT <= p.n) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      if (i >= rows) break;
+  for (int j = 0; j < NT; j += 2) {
+    const int64_t at = n + 16 * j;
+    if (at >= p.n) break;
+    float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (p.bias) {
 #pragma unroll
-      for (int j = 0; j < NT; j += 2) {
-        const f32x4 u = acc[i][j] + bias[j], v = acc[i][j + 1] + bias[j + 1];
-        Wide<sizeof(B)>::store(out + 4 * j, u32x4{pack2<O>(u[0], u[1]), pack2<O>(u[2], u[3]), pack2<O>(v[0], v[1]),
-                                                  pack2<O>(v[2], v[3])});
-      }
-      out += p.pitch;
+      for (int r = 0; r < 8; ++r) bias[r] = load_f32<O>(((const B*)p.bias)[min(at + r, p.n - 1)]);
     }
-  } else {
-    const int cols = (int)(p.n - n);
+    B* out = (B*)p.out + m * p.pitch + at;
+    if (at + 8 <= p.n) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      if (i >= rows) break;
+      for (int i = 0; i < MT; ++i) {
+        if (i >= rows) break;
+        const f32x4 u = acc[i][j], v = acc[i][j + 1];
+        Wide<sizeof(B)>::store(out, u32x4{pack2<O>(u[0] + bias[0], u[1] + bias[1]), pack2<O>(u[2] + bias[2], u[3] + bias[3]),
+                                          pack2<O>(v[0] + bias[4], v[1] + bias[5]), pack2<O>(v[2] + bias[6], v[3] + bias[7])});
+        out += p.pitch;
+      }
+    } else {
+      const int cols = (int)(p.n - at);
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int i = 0; i < MT; ++i) {
+        if (i >= rows) break;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (4 * j + r < cols) out[4 * j + r] = store_bits<O>(acc[i][j][r] + bias[j][r]);
-      out += p.pitch;
+        for (int r = 0; r < 7; ++r)
+          if (r < cols) out[r] = store_bits<O>((r < 4 ? acc[i][j][r & 3] : acc[i][j + 1][r & 3]) + bias[r]);
+        out += p.pitch;
+      }
     }
   }
 }
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 2 : 1) void k_til
   const int64_t m0 = (int64_t)tm * T::BM, n0 = (int64_t)tn * T::BN;
   Loader<T> loader(p, lds, m0, n0, wave, lane);
 
-  const int64_t m = m0 + wm * 16 * MT + c * MT, n = n0 + wn * 16 * NT + g * 4 * NT;
+  const int64_t m = m0 + wm * 16 * MT + c * MT, n = n0 + wn * 16 * NT;
   const int64_t sa_at = min(m, p.sa_pitch - 8);       // rows past the end take scales of the last ones
   const int64_t sb_at = min(n0 + wn * 16 * NT, p.n - 1) / kBlockK * p.kb;
   Scales<POW2> sa;
@@ -287,9 +287,9 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 2 : 1) void k_til
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const uint8_t* la = lds + (wm * 16 * MT + c * MT) * kBlockK;
-  const uint8_t* lb = lds + T::BM * kBlockK + (wn * 16 * NT + (c >> 2) * 4 * NT + (c & 3)) * kBlockK;
-  const int piece0 = (g ^ (c & 7)) * 16, piece1 = piece0 ^ 64;
+  const uint8_t* la = lds + (wm * 16 * MT + c) * kBlockK;
+  const uint8_t* lb = lds + T::BM * kBlockK + (wn * 16 * NT + c) * kBlockK;
+  const int piece0 = (g ^ (c >> 1)) * 16, piece1 = piece0 ^ 64;
 
   loader.fetch(0, 0);
   scales(0);
@@ -309,14 +309,14 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 2 : 1) void k_til
     i32x8 w[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      const i32x4 x = *(const i32x4*)(lb + buf + j * 4 * kBlockK + piece0);
-      const i32x4 y = *(const i32x4*)(lb + buf + j * 4 * kBlockK + piece1);
+      const i32x4 x = *(const i32x4*)(lb + buf + j * 16 * kBlockK + piece0);
+      const i32x4 y = *(const i32x4*)(lb + buf + j * 16 * kBlockK + piece1);
       w[j] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     auto row = [&](auto I) {
       constexpr int i = decltype(I)::value;
-      const i32x4 x = *(const i32x4*)(la + buf + i * kBlockK + piece0);
-      const i32x4 y = *(const i32x4*)(la + buf + i * kBlockK + piece1);
+      const i32x4 x = *(const i32x4*)(la + buf + i * 16 * kBlockK + piece0);
+      const i32x4 y = *(const i32x4*)(la + buf + i * 16 * kBlockK + piece1);
       const i32x8 v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
@@ -334,7 +334,7 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 2 : 1) void k_til
     each<MT>(row);
   }
 
-  store_tile<MT, NT, O>(p, acc, m, n);
+  store_tile<MT, NT, O>(p, acc, m, n, g);
 }
 
 // 256 x 256 for e8m0 scales with four waves of 128 x 128, one to a SIMD: the matrix instruction applies
@@ -377,11 +377,11 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
   int tm, tn;
   if (!tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn)) return;
   const int64_t m0 = (int64_t)tm * Q::BM, n0 = (int64_t)tn * Q::BN, kp = (int64_t)p.kb * kBlockK;
-  const int64_t m = m0 + wm * 128 + c * 8, n = n0 + wn * 128 + g * 32;
+  const int64_t m = m0 + wm * 128 + c * 8, n = n0 + wn * 128;
   const int last = p.kb - 1;
 
-  // LDS rows of a part: x: 64 * wm + 4 * c + i for row 128 * wm + 8 * c + 4 * part + i,
-  // w: 64 * wn + 16 * (c / 4) + 4 * j + c % 4 for column 128 * wn + 32 * (c / 4) + 16 * part + 4 * j + c % 4
+  // LDS rows of a part: 64 * wm + 16 * i + c holds the row that lane c reads as piece i, row
+  // 128 * wm + 8 * c + 4 * part + i; the columns' likewise
   const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   const u32x4 rx = buffer_of(p.a + m0 * kp), rw = buffer_of(p.b + n0 * kp);
   uint32_t vx[8], vw[8];
@@ -390,11 +390,11 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = (wave + 4 * i) * 8 + lane / 8;              // of the part, in LDS
-      const int64_t xm = (row >> 6) * 128 + (row >> 2 & 15) * 8 + part * 4 + (row & 3);
-      const int64_t wc = (row >> 6) * 128 + (row >> 4 & 3) * 32 + part * 16 + (row & 15);
-      const int kx = row >> 2 & 7, kw = (row & 3) | (row >> 4 & 1) << 2;
-      vx[part * 4 + i] = (uint32_t)(min(xm, p.m - 1 - m0) * kp + ((lane & 7) ^ kx) * 16);
-      vw[part * 4 + i] = (uint32_t)(min(wc, p.n - 1 - n0) * kp + ((lane & 7) ^ kw) * 16);
+      const int64_t xm = (row >> 6) * 128 + (row & 15) * 8 + part * 4 + (row >> 4 & 3);
+      const int64_t wc = (row >> 6) * 128 + column_of(part * 4 + (row >> 4 & 3), row & 15);
+      const int key = row >> 1 & 7;
+      vx[part * 4 + i] = (uint32_t)(min(xm, p.m - 1 - m0) * kp + ((lane & 7) ^ key) * 16);
+      vw[part * 4 + i] = (uint32_t)(min(wc, p.n - 1 - n0) * kp + ((lane & 7) ^ key) * 16);
     }
   const uint32_t vs = (uint32_t)min((int64_t)lane * 4, p.sa_pitch - 4 - m0);
   auto load_x = [&](int part, int i, int k) {
@@ -410,16 +410,16 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
     load_lds<4>(rs, vs, 0, base + Q::kScales + ((k & 3) * 4 + wave) * 256);
   };
 
-  const int piece = (g ^ (c & 7)) * 16;
-  const uint8_t* lx = lds + (wm * 64 + c * 4) * kBlockK;
-  const uint8_t* lw = lds + 2 * Q::kPart + (wn * 64 + (c >> 2) * 16 + (c & 3)) * kBlockK;
+  const int piece = (g ^ (c >> 1)) * 16;
+  const uint8_t* lx = lds + (wm * 64 + c) * kBlockK;
+  const uint8_t* lw = lds + 2 * Q::kPart + (wn * 64 + c) * kBlockK;
   const uint8_t* ls = lds + Q::kScales + wave * 256 + wm * 128 + c * 8;
   i32x4 x[8][2], w[8][2];            // [piece][half of its 32 bytes]
   auto read_x = [&](int k, int i, int h) {
-    x[i][h] = *(const i32x4*)(lx + (k & 1) * Q::kStep + (i >> 2) * Q::kPart + (i & 3) * kBlockK + (h ? piece ^ 64 : piece));
+    x[i][h] = *(const i32x4*)(lx + (k & 1) * Q::kStep + (i >> 2) * Q::kPart + (i & 3) * 16 * kBlockK + (h ? piece ^ 64 : piece));
   };
   auto read_w = [&](int k, int j, int h) {
-    w[j][h] = *(const i32x4*)(lw + (k & 1) * Q::kStep + (j >> 2) * Q::kPart + (j & 3) * 4 * kBlockK + (h ? piece ^ 64 : piece));
+    w[j][h] = *(const i32x4*)(lw + (k & 1) * Q::kStep + (j >> 2) * Q::kPart + (j & 3) * 16 * kBlockK + (h ? piece ^ 64 : piece));
   };
 
   // the columns' scales of 256 steps: four in each lane
@@ -503,7 +503,7 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
     });
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing may reach LDS after the workgroup's end
-  store_tile<8, 8, O>(p, acc, m, n);
+  store_tile<8, 8, O>(p, acc, m, n, g);
 }
 
 template <typename T, typename O>
