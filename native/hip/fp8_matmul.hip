@@ -458,6 +458,9 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
   for (int i = 0; i < 4; ++i) read_x(0, i, 0), read_x(0, i, 1);
 #pragma unroll
   for (int j = 0; j < 4; ++j) read_w(0, j, 0), read_w(0, j, 1);
+  // Nothing is pending where the loop begins, so that in it the compiler waits for what it needs alone
+  // (0xC07F: lgkmcnt 0, the other counters at their most).
+  __builtin_amdgcn_s_waitcnt(0xC07F);
 
 #pragma unroll 1
   for (int k = 0; k < p.kb; ++k) {
@@ -481,29 +484,178 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
     meet<22>();
     now = next;
     quarter(Index<0>{}, Index<0>{}, [&](int at) {
-      if (at < 8) read_w(k, 4 + at / 2, at % 2);
-      if (at % 4 == 2) load_x(0, at / 4, k + 2);
+      if (at % 2 == 0) read_w(k, 4 + at / 4, at / 2 % 2);
+      if (at % 4 == 1) load_x(0, at / 4, k + 2);
     });
     meet<21>();
     quarter(Index<0>{}, Index<1>{}, [&](int at) {
-      if (at < 8) read_x(k, 4 + at / 2, at % 2);
-      if (at % 4 == 2) load_w(0, at / 4, k + 2);
+      if (at % 2 == 0) read_x(k, 4 + at / 4, at / 2 % 2);
+      if (at % 4 == 1) load_w(0, at / 4, k + 2);
     });
     meet<21>();
     quarter(Index<1>{}, Index<1>{}, [&](int at) {
-      if (at < 8) read_x(k + 1, at / 2, at % 2);
-      if (at % 4 == 2) load_w(1, at / 4, k + 2);
+      if (at % 2 == 0) read_x(k + 1, at / 4, at / 2 % 2);
+      if (at % 4 == 1) load_w(1, at / 4, k + 2);
     });
     meet<21>();
     next = *(const uint2*)(ls + (k + 1 & 3) * 1024);
     quarter(Index<1>{}, Index<0>{}, [&](int at) {
       if (at == 0) load_s(k + 3);
-      if (at % 4 == 2) load_x(1, at / 4, k + 2);
-      if (at % 4 == 3) read_w(k + 1, at / 4, 0), read_w(k + 1, at / 4, 1);
+      if (at % 4 == 1) load_x(1, at / 4, k + 2);
+      if (at % 4 == 3) read_w(k + 1, at / 4, 0);
+      if (at % 4 == 0 && at) read_w(k + 1, at / 4 - 1, 1);
+      if (at == 15) read_w(k + 1, 3, 1);
     });
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing may reach LDS after the workgroup's end
   store_tile<8, 8, O>(p, acc, m, n, g);
+}
+
+// 256 x 256 for float scales with eight waves of 128 x 64, two to a SIMD. A block's sum leaves the matrix instruction
+// and enters the float32 sum by a multiply-add with its scale, 4 of them to a product of 32 cycles: the
+// vector units take half as long as the matrix units, next to them. The multiply-adds stay two products behind.
+//
+// A step is eight pieces of rows times four of columns. The next step's operands are read from LDS as
+// registers fall free, and each part of LDS is filled again, for the step after the next, once every wave has read it:
+//   piece 0 | 1 .. 4 | 5 6 7     "|": all waves meet; x[i] is read after piece i - 4, w[j] in piece 7
+//   after the first meeting   w(k+2) and rows' pieces 0-3 (k+2)    (read in step k-1)
+//   after the second          rows' pieces 4-7 (k+2), rows' scales (k+3)
+// so a load has a step and a half to arrive. Each wave counts its own loads: 6 and 3.
+struct Eight {
+  static constexpr int BM = 256, BN = 256, kThreads = 512;
+  static constexpr int kRows = 128 * kBlockK;                     // half of the rows' pieces: 16 KB
+  static constexpr int kStep = 4 * kRows, kScales = 2 * kStep;    // then 4 steps x 256 scales
+  static constexpr int kLds = kScales + 4 * 1024;
+};
+
+template <typename O>
+__global__ __launch_bounds__(512, 2) void k_eight(MatArgs p, int tiles_m, int tiles_n) {
+  using Q = Eight;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Q::kLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4, wm = wave >> 2, wn = wave & 3;
+  int tm, tn;
+  if (!tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn)) return;
+  const int64_t m0 = (int64_t)tm * Q::BM, n0 = (int64_t)tn * Q::BN, kp = (int64_t)p.kb * kBlockK;
+  const int64_t m = m0 + wm * 128 + c * 8, n = n0 + wn * 64;
+  const int last = p.kb - 1;
+
+  // LDS rows: rows' half h: 64 * wm + 16 * i + c holds row 128 * wm + 8 * c + 4 * h + i; columns: 64 * wn + 16 * j + c
+  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  const u32x4 rx = buffer_of(p.a + m0 * kp), rw = buffer_of(p.b + n0 * kp);
+  uint32_t vx[4], vw[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = (wave + 8 * (i & 1)) * 8 + lane / 8;
+    const int64_t at = (row >> 6) * 128 + (row & 15) * 8 + (i >> 1) * 4 + (row >> 4 & 3);
+    vx[i] = (uint32_t)(min(at, p.m - 1 - m0) * kp + ((lane & 7) ^ (row >> 1 & 7)) * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = (wave + 8 * i) * 8 + lane / 8;
+    const int64_t at = (row >> 6) * 64 + column_of(row >> 4 & 3, row & 15);
+    vw[i] = (uint32_t)(min(at, p.n - 1 - n0) * kp + ((lane & 7) ^ (row >> 1 & 7)) * 16);
+  }
+  auto load_x = [&](int half, int i, int k) {
+    load_lds<16>(rx, vx[half * 2 + i], min(k, last) * kBlockK,
+                 base + (k & 1) * Q::kStep + half * Q::kRows + (wave + 8 * i) * 1024);
+  };
+  auto load_w = [&](int i, int k) {
+    load_lds<16>(rw, vw[i], min(k, last) * kBlockK, base + (k & 1) * Q::kStep + 2 * Q::kRows + (wave + 8 * i) * 1024);
+  };
+  const uint32_t vs = (uint32_t)min((int64_t)(wave & 3) * 64 + lane, p.sa_pitch - 1 - m0) * 4;
+  auto load_s = [&](int k) {                                      // waves 4-7 write the same once more
+    const u32x4 rs = buffer_of((const float*)p.sa + m0 + min(k, last) * p.sa_pitch);
+    load_lds<4>(rs, vs, 0, base + Q::kScales + (k & 3) * 1024 + (wave & 3) * 256);
+  };
+
+  const int piece = (g ^ (c >> 1)) * 16;
+  const uint8_t* lx = lds + (wm * 64 + c) * kBlockK;
+  const uint8_t* lw = lds + 2 * Q::kRows + (wn * 64 + c) * kBlockK;
+  const uint8_t* ls = lds + Q::kScales + wm * 512 + c * 32;
+  i32x4 x[4][2], w[4][2];            // [piece % 4][half of its 32 bytes]
+  auto read_x = [&](int k, int i, int h) {
+    x[i & 3][h] = *(const i32x4*)(lx + (k & 1) * Q::kStep + (i >> 2) * Q::kRows + (i & 3) * 16 * kBlockK + (h ? piece ^ 64 : piece));
+  };
+  auto read_w = [&](int k, int j, int h) {
+    w[j][h] = *(const i32x4*)(lw + (k & 1) * Q::kStep + j * 16 * kBlockK + (h ? piece ^ 64 : piece));
+  };
+
+  // the columns' scales of 64 steps: one in each lane
+  const float* sb = (const float*)p.sb + min(n, p.n - 1) / kBlockK * p.kb;
+  float sbs = sb[min(lane, last)];
+  asm volatile("" : "+v"(sbs));
+
+  f32x4 acc[8][4], t[4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  load_s(0), load_s(1);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_w(i, k);
+    load_x(0, 0, k), load_x(0, 1, k);
+    load_x(1, 0, k), load_x(1, 1, k);
+    load_s(k + 2);
+  }
+  meet<12>();
+  f32x4 next[2] = {*(const f32x4*)ls, *(const f32x4*)(ls + 16)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) read_x(0, i, 0), read_x(0, i, 1);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) read_w(0, j, 0), read_w(0, j, 1);
+  __builtin_amdgcn_s_waitcnt(0xC07F);           // as in k_quarters
+
+#pragma unroll 1
+  for (int k = 0; k < p.kb; ++k) {
+    if ((k & 63) == 0 && k) {
+      sbs = sb[min(k + lane, last)];
+      asm volatile("" : "+v"(sbs));
+    }
+    const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sbs), k & 63));
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = next[i >> 2][i & 3] * ws;
+    auto add = [&](auto At) {
+      constexpr int at = decltype(At)::value, i = at / 4, j = at % 4;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[j][r], s[i], acc[i][j][r]);
+    };
+    auto one = [&](auto At) {
+      constexpr int at = decltype(At)::value, i = at / 4, j = at % 4;
+      const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+      t[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(w[j]), join(x[i & 3]), zero, 0, 0, 0, 0, 0, 0);
+      if constexpr (at >= 2) add(Index<at - 2>{});
+      if constexpr (at == 3) meet<9>();
+      if constexpr (at == 19) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        meet<9>();
+      }
+      if constexpr (i < 4) {
+        if constexpr (j == 3) read_x(k, i + 4, 0), read_x(k, i + 4, 1);
+      } else {
+        if constexpr (j == 3) read_x(k + 1, i - 4, 0), read_x(k + 1, i - 4, 1);
+        if constexpr (i == 7) read_w(k + 1, j, 0), read_w(k + 1, j, 1);
+      }
+      if constexpr (at == 5 || at == 7 || at == 9 || at == 11) load_w((at - 5) / 2, k + 2);
+      if constexpr (at == 13 || at == 15) load_x(0, (at - 13) / 2, k + 2);
+      if constexpr (at == 21 || at == 23) load_x(1, (at - 21) / 2, k + 2);
+      if constexpr (at == 25) {
+        load_s(k + 4);
+        next[0] = *(const f32x4*)(ls + (k + 1 & 3) * 1024);
+        next[1] = *(const f32x4*)(ls + (k + 1 & 3) * 1024 + 16);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    each<32>(one);
+    add(Index<30>{});
+    add(Index<31>{});
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing may reach LDS after the workgroup's end
+  store_tile<8, 4, O>(p, acc, m, n, g);
 }
 
 template <typename T, typename O>
@@ -519,10 +671,12 @@ int run_tile(const MatArgs& p, bool pow2, hipStream_t s) {
 using Big = Tile<8, 4, 2, 4>;
 
 template <typename O>
-int run_quarters(const MatArgs& p, hipStream_t s) {
+int run_256(const MatArgs& p, bool pow2, hipStream_t s) {
   const int64_t tm = (p.m + 255) / 256, tn = (p.n + 255) / 256, total = tm * tn;
   if (total > (1 << 30)) return -1;
-  k_quarters<O><<<(unsigned)((total + 7) / 8 * 8), 256, 0, s>>>(p, (int)tm, (int)tn);
+  const unsigned grid = (unsigned)((total + 7) / 8 * 8);
+  if (pow2) k_quarters<O><<<grid, 256, 0, s>>>(p, (int)tm, (int)tn);
+  else k_eight<O><<<grid, 512, 0, s>>>(p, (int)tm, (int)tn);
   return (int)hipGetLastError();
 }
 
@@ -538,7 +692,7 @@ int run_simple(const MatArgs& p, bool pow2, hipStream_t s) {
 
 template <typename O>
 int run(const MatArgs& p, bool pow2, hipStream_t s) {
-  if (p.m > 64) return pow2 ? run_quarters<O>(p, s) : run_tile<Big, O>(p, pow2, s);
+  if (p.m > 64) return run_256<O>(p, pow2, s);
   return run_simple<O>(p, pow2, s);
 }
 
