@@ -680,6 +680,325 @@ int run_256(const MatArgs& p, bool pow2, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
+// Four neighbours of row m from column n (a multiple of 4) on, plus bias.
+template <typename O>
+__device__ __forceinline__ void store4(const MatArgs& p, f32x4 v, int64_t m, int64_t n) {
+  using B = typename Bits<O>::type;
+  typedef uint32_t u32x2_at2 __attribute__((ext_vector_type(2), aligned(2)));
+  B* out = (B*)p.out + m * p.pitch + n;
+  if (p.bias) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] += load_f32<O>(((const B*)p.bias)[min(n + r, p.n - 1)]);
+  }
+  if (n + 4 <= p.n) {
+    *(u32x2_at2*)out = u32x2_at2{pack2<O>(v[0], v[1]), pack2<O>(v[2], v[3])};
+  } else {
+#pragma unroll
+    for (int r = 0; r < 3; ++r)
+      if (n + r < p.n) out[r] = store_bits<O>(v[r]);
+  }
+}
+
+// ---------------------------------------------------------------- 128 x 128, K in parts
+//
+// For products with too few tiles of 256 x 256 to fill the card: four waves of 64 x 64, a ring of STAGES steps in LDS, and
+// K in gridDim.y parts whose float32 sums go to a workspace and are joined by k_join in the order of the parts. With two
+// stages (66 KB) two workgroups share a CU and run while the other waits; with four, one has three steps of loads in flight.
+struct Mid {
+  static constexpr int BM = 128, BN = 128, kThreads = 256;
+  static constexpr int kTile = 128 * kBlockK;                     // rows' or columns' step: 16 KB
+  static constexpr int kStage = 2 * kTile + 4 * 256;              // and each wave's rows' scales
+  static constexpr int kLoads = 9;                                // of a wave and step
+};
+
+template <int STAGES, typename O, bool POW2>
+__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void k_mid(MatArgs p, int tiles_m, int tiles_n, float* parts) {
+  using Q = Mid;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * Q::kStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
+  int tm, tn;
+  if (!tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn)) return;
+  const int64_t m0 = (int64_t)tm * Q::BM, n0 = (int64_t)tn * Q::BN, kp = (int64_t)p.kb * kBlockK;
+  const int64_t m = m0 + wm * 64 + c * 4, n = n0 + wn * 64;
+  const int first = (int)((int64_t)p.kb * blockIdx.y / gridDim.y), end = (int)((int64_t)p.kb * (blockIdx.y + 1) / gridDim.y);
+
+  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  const u32x4 rx = buffer_of(p.a + m0 * kp), rw = buffer_of(p.b + n0 * kp);
+  uint32_t vx[4], vw[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = (wave + 4 * i) * 8 + lane / 8, key = row >> 1 & 7, half = (row >> 6) * 64, at = row >> 4 & 3;
+    vx[i] = (uint32_t)(min((int64_t)half + (row & 15) * 4 + at, p.m - 1 - m0) * kp + ((lane & 7) ^ key) * 16);
+    vw[i] = (uint32_t)(min((int64_t)half + column_of(at, row & 15), p.n - 1 - n0) * kp + ((lane & 7) ^ key) * 16);
+  }
+  constexpr int kScale = POW2 ? 1 : 4;
+  // the wave's rows' scales: 64 floats, or bytes from the tile's first row on
+  const uint32_t vs = POW2 ? (uint32_t)min((int64_t)lane * 4, p.sa_pitch - 4 - m0)
+                           : (uint32_t)min((int64_t)wm * 64 + lane, p.sa_pitch - 1 - m0) * 4;
+  auto fetch = [&](int k, int stage) {
+    const uint32_t to = base + stage * Q::kStage;
+    const u32x4 rs = buffer_of((const uint8_t*)p.sa + (m0 + k * p.sa_pitch) * kScale);
+    load_lds<4>(rs, vs, 0, to + 2 * Q::kTile + wave * 256);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_lds<16>(rx, vx[i], k * kBlockK, to + (wave + 4 * i) * 1024);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_lds<16>(rw, vw[i], k * kBlockK, to + Q::kTile + (wave + 4 * i) * 1024);
+  };
+
+  const int piece = (g ^ (c >> 1)) * 16;
+  const uint8_t* lx = lds + (wm * 64 + c) * kBlockK;
+  const uint8_t* lw = lds + Q::kTile + (wn * 64 + c) * kBlockK;
+  const uint8_t* ls = lds + 2 * Q::kTile + wave * 256 + (POW2 ? wm * 64 + c * 4 : c * 16);
+
+  // the columns' scales: of 256 steps, four bytes in a lane, or of 64, a float in a lane
+  constexpr int kChunk = POW2 ? 256 : 64;
+  const int64_t sb_at = min(n, p.n - 1) / kBlockK * p.kb;
+  auto column_scales = [&](int k) {
+    uint32_t v = 0;
+    if constexpr (POW2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v |= (uint32_t)((const uint8_t*)p.sb)[sb_at + min(k + lane * 4 + i, end - 1)] << (8 * i);
+    } else {
+      v = ((const uint32_t*)p.sb)[sb_at + min(k + lane, end - 1)];
+    }
+    asm volatile("" : "+v"(v));
+    return v;
+  };
+  uint32_t sbs = column_scales(first);
+
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+  for (int d = 0; d < STAGES - 1; ++d)
+    if (first + d < end) fetch(first + d, d);
+  int stage = 0;
+#pragma unroll 1
+  for (int k = first; k < end; ++k) {
+    const int done = k - first;
+    if (done && done % kChunk == 0) sbs = column_scales(k);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the last step's reads
+    if (k + STAGES - 2 < end) meet<(STAGES - 2) * Q::kLoads>();
+    else meet<0>();
+    if (k + STAGES - 1 < end) fetch(k + STAGES - 1, stage ? stage - 1 : STAGES - 1);
+    const int at = stage * Q::kStage;
+    i32x4 x[4][2], w[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        w[j][h] = *(const i32x4*)(lw + at + j * 16 * kBlockK + (h ? piece ^ 64 : piece));
+        x[j][h] = *(const i32x4*)(lx + at + j * 16 * kBlockK + (h ? piece ^ 64 : piece));
+      }
+    uint32_t xb = 0, wb = 0;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (POW2) {
+      xb = *(const uint32_t*)(ls + at);
+      wb = __builtin_amdgcn_readlane(sbs, done >> 2 & 63) >> (8 * (done & 3));
+    } else {
+      s = *(const f32x4*)(ls + at) * __uint_as_float(__builtin_amdgcn_readlane(sbs, done & 63));
+    }
+    auto row = [&](auto I) {
+      constexpr int i = decltype(I)::value;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (POW2) {
+          acc[i][j] = mfma_scaled<i>(join(w[j]), join(x[i]), acc[i][j], wb, xb);
+        } else {
+          const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+          const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(w[j]), join(x[i]), zero, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[r], s[i], acc[i][j][r]);
+        }
+      }
+    };
+    each<4>(row);
+    stage = stage + 1 < STAGES ? stage + 1 : 0;
+  }
+  if (!parts) {
+    store_tile<4, 4, O>(p, acc, m, n, g);
+    return;
+  }
+  // this part's sums, float32, rows of n up to a multiple of 4
+  const int64_t wide = (p.n + 3) / 4 * 4;
+  float* out = parts + ((int64_t)blockIdx.y * p.m + m) * wide;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (m + i >= p.m) break;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t at = n + g * 8 + (j >> 1) * 32 + (j & 1) * 4;
+      if (at < p.n) *(f32x4*)(out + i * wide + at) = acc[i][j];
+    }
+  }
+}
+
+// out = the sum of the parts in their order, plus bias: four neighbours a lane.
+template <typename O>
+__global__ __launch_bounds__(256) void k_join(MatArgs p, const float* parts, int count) {
+  const int64_t quads = (p.n + 3) / 4, m = blockIdx.y, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= quads) return;
+  const f32x4* in = (const f32x4*)parts + m * quads + at;
+  f32x4 v = in[0];
+  for (int i = 1; i < count; ++i) v += in[i * p.m * quads];
+  store4<O>(p, v, m, at * 4);
+}
+
+template <typename O>
+int run_mid(const MatArgs& p, bool pow2, int count, float* parts, hipStream_t s) {
+  const int64_t tm = (p.m + 127) / 128, tn = (p.n + 127) / 128, total = tm * tn;
+  if (total > (1 << 30) || count > 65535) return -1;
+  const dim3 grid((unsigned)((total + 7) / 8 * 8), count);
+  float* to = count > 1 ? parts : nullptr;
+  if (total * count > 256) {
+    if (pow2) k_mid<2, O, true><<<grid, 256, 0, s>>>(p, (int)tm, (int)tn, to);
+    else k_mid<2, O, false><<<grid, 256, 0, s>>>(p, (int)tm, (int)tn, to);
+  } else {
+    if (pow2) k_mid<4, O, true><<<grid, 256, 0, s>>>(p, (int)tm, (int)tn, to);
+    else k_mid<4, O, false><<<grid, 256, 0, s>>>(p, (int)tm, (int)tn, to);
+  }
+  if (count > 1) {
+    const int64_t gx = ((p.n + 3) / 4 + 255) / 256;
+    if (gx > 0x7FFFFFFF || p.m > 65535) return -1;
+    k_join<O><<<dim3((unsigned)gx, (unsigned)p.m), 256, 0, s>>>(p, parts, count);
+  }
+  return (int)hipGetLastError();
+}
+
+// ---------------------------------------------------------------- few rows
+//
+// Up to 128 rows the weight's bytes are what counts: one workgroup takes all rows and 16 * NP columns, its waves
+// take every WAVES-th block of K and read their operands from memory straight into registers, DEPTH
+// blocks ahead, each weight byte once on the whole card; the rows are read again by each workgroup, out of L2.
+// No wave waits for another until the end, when the waves' sums are added through LDS in the order of
+// the waves. Rows m = c * MP + i as in the tiles; columns as in column_of where NP is 2.
+template <int MP, int NP, int WAVES, int DEPTH, typename O, bool POW2>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_narrow(MatArgs p) {
+  __shared__ f32x4 part[WAVES * MP * NP * 64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16 * NP, kp = (int64_t)p.kb * kBlockK;
+  const uint8_t *px[MP], *pw[NP];
+#pragma unroll
+  for (int i = 0; i < MP; ++i) px[i] = p.a + min((int64_t)c * MP + i, p.m - 1) * kp + g * 16;
+#pragma unroll
+  for (int j = 0; j < NP; ++j) pw[j] = p.b + min(n0 + (NP == 2 ? column_of(j, c) : c), p.n - 1) * kp + g * 16;
+  const int64_t sa_at = min((int64_t)c * MP, p.sa_pitch - MP), sb_at = n0 / kBlockK * p.kb;
+
+  struct Block {
+    i32x4 x[MP][2], w[NP][2];
+    float xs[MP], ws;
+    uint32_t xb[MP > 4 ? 2 : 1], wb;
+  };
+  auto load = [&](Block& b, int kb) {
+    const int64_t at = (int64_t)kb * kBlockK;
+#pragma unroll
+    for (int j = 0; j < NP; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) b.w[j][h] = *(const i32x4*)(pw[j] + at + 64 * h);
+#pragma unroll
+    for (int i = 0; i < MP; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) b.x[i][h] = *(const i32x4*)(px[i] + at + 64 * h);
+    const int64_t s = kb * p.sa_pitch + sa_at;
+    if constexpr (POW2) {
+      const uint8_t* q = (const uint8_t*)p.sa + s;
+      if constexpr (MP == 1) b.xb[0] = *q;
+      else if constexpr (MP == 2) b.xb[0] = *(const uint16_t*)q;
+      else if constexpr (MP == 4) b.xb[0] = *(const uint32_t*)q;
+      else b.xb[0] = ((const uint32_t*)q)[0], b.xb[1] = ((const uint32_t*)q)[1];
+      b.wb = ((const uint8_t*)p.sb)[sb_at + kb];
+    } else {
+#pragma unroll
+      for (int i = 0; i < MP; ++i) b.xs[i] = ((const float*)p.sa)[s + i];
+      b.ws = ((const float*)p.sb)[sb_at + kb];
+    }
+  };
+
+  f32x4 acc[MP][NP];
+#pragma unroll
+  for (int i = 0; i < MP; ++i)
+#pragma unroll
+    for (int j = 0; j < NP; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto use = [&](const Block& b) {
+    auto piece = [&](auto I) {
+      constexpr int i = decltype(I)::value;
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        if constexpr (POW2) {
+          acc[i][j] = mfma_scaled<i & 3>(join(b.w[j]), join(b.x[i]), acc[i][j], b.wb, b.xb[i >> 2]);
+        } else {
+          const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+          const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(b.w[j]), join(b.x[i]), zero, 0, 0, 0, 0, 0, 0);
+          const float s = b.xs[i] * b.ws;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[r], s, acc[i][j][r]);
+        }
+      }
+    };
+    each<MP>(piece);
+  };
+
+  // Rows a power of two apart lie on one memory channel, so workgroups that walk K in step would ask few
+  // channels at a time: each begins at a block of its own and goes round.
+  const int first = blockIdx.x % p.kb;
+  auto block = [&](int q) {
+    const int kb = min(q, p.kb - 1) + first;
+    return kb < p.kb ? kb : kb - p.kb;
+  };
+  Block ring[DEPTH];
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) {
+    load(ring[d], block(wave + d * WAVES));     // past the end: the last one, not used
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  int q = wave;
+#pragma unroll 1
+  for (; q + (2 * DEPTH - 1) * WAVES < p.kb; q += DEPTH * WAVES) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      use(ring[d]);
+      load(ring[d], block(q + (d + DEPTH) * WAVES));
+      __builtin_amdgcn_sched_barrier(0);        // or all DEPTH loads end up behind all uses, and are waited for at once
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) {
+    if (q + d * WAVES < p.kb) use(ring[d]);
+    if (q + (d + DEPTH) * WAVES < p.kb) load(ring[d], block(q + (d + DEPTH) * WAVES));
+  }
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d)
+    if (q + (d + DEPTH) * WAVES < p.kb) use(ring[d]);
+
+#pragma unroll
+  for (int i = 0; i < MP; ++i)
+#pragma unroll
+    for (int j = 0; j < NP; ++j) part[(wave * MP * NP + i * NP + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < MP * NP * 64; e += 64 * WAVES) {
+    f32x4 v = part[e];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) v += part[w * MP * NP * 64 + e];
+    const int l = e & 63, i = e / 64 / NP, j = e / 64 % NP;
+    const int64_t m = (int64_t)(l & 15) * MP + i, n = n0 + (NP == 2 ? (l >> 4) * 8 + j * 4 : (l >> 4) * 4);
+    if (m < p.m && n < p.n) store4<O>(p, v, m, n);
+  }
+}
+
+template <int MP, int NP, int WAVES, int DEPTH, typename O>
+int narrow(const MatArgs& p, bool pow2, hipStream_t s) {
+  const int64_t grid = (p.n + 16 * NP - 1) / (16 * NP);
+  if (grid > 0x7FFFFFFF) return -1;
+  if (pow2) k_narrow<MP, NP, WAVES, DEPTH, O, true><<<(unsigned)grid, 64 * WAVES, 0, s>>>(p);
+  else k_narrow<MP, NP, WAVES, DEPTH, O, false><<<(unsigned)grid, 64 * WAVES, 0, s>>>(p);
+  return (int)hipGetLastError();
+}
+
 template <typename O>
 int run_simple(const MatArgs& p, bool pow2, hipStream_t s) {
   const int64_t gx = (p.n + 63) / 64, gy = (p.m + 15) / 16;
@@ -692,8 +1011,11 @@ int run_simple(const MatArgs& p, bool pow2, hipStream_t s) {
 
 template <typename O>
 int run(const MatArgs& p, bool pow2, hipStream_t s) {
-  if (p.m > 64) return run_256<O>(p, pow2, s);
-  return run_simple<O>(p, pow2, s);
+  if (p.m > 128) return run_256<O>(p, pow2, s);
+  if (p.m <= 16) return p.n >= 8192 ? narrow<1, 2, 8, 4, O>(p, pow2, s) : narrow<1, 1, 8, 4, O>(p, pow2, s);
+  if (p.m <= 32) return p.n >= 8192 ? narrow<2, 2, 8, 4, O>(p, pow2, s) : narrow<2, 1, 8, 4, O>(p, pow2, s);
+  if (p.m <= 64) return narrow<4, 2, 8, 3, O>(p, pow2, s);
+  return narrow<8, 2, 8, 2, O>(p, pow2, s);
 }
 
 }  // namespace
