@@ -5,7 +5,7 @@
 // row of bytes starts on a 128-byte line and no product has a tail along K.
 //   values  [R][Kp] bytes
 //   scales  1 x 128:   [Kp/128][R up to a multiple of 8]   block by block: the rows of a tile are neighbours
-//           128 x 128: [ceil(R/128)][Kp/128]
+//           128 x 128: [ceil(R/128)][Kp/128 up to a multiple of 4]
 // A scale is a float32 (largest magnitude / 448) or an e8m0 byte b that stands for 2^(b-127).
 #pragma once
 #include <hip/hip_bf16.h>

@@ -282,7 +282,7 @@ __global__ __launch_bounds__(kThreads) void k_tiles(QuantArgs a) {
     const int64_t r = r0 + p * kRowsAtOnce;
     if (r < a.rows) *(uint2*)((uint8_t*)a.values + r * (int64_t)a.padded + c) = to_e4m3(v[p], inv);
   }
-  if (threadIdx.x == 0) put_scale<POW2>(a.scales, rb * kb + cb, s);
+  if (threadIdx.x == 0) put_scale<POW2>(a.scales, rb * ((kb + 3) / 4 * 4) + cb, s);
 }
 
 int padded_cols(int cols) { return (cols + kBlockK - 1) / kBlockK * kBlockK; }

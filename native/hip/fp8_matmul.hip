@@ -7,16 +7,18 @@
 // inputs, against 1.7e-3 for a bf16 output's rounding; float32 outputs are not offered for it.
 #include "fp8_blocks.h"
 
+#include <algorithm>
+
 namespace yoda_fp8 {
 namespace {
 
 struct MatArgs {
   const uint8_t *a, *b;                // [M][Kp], [N][Kp]
-  const void *sa, *sb;                 // [Kp/128][sa_pitch], [ceil(N/128)][Kp/128]
+  const void *sa, *sb;                 // [Kp/128][sa_pitch], [ceil(N/128)][Kp/128 up to a multiple of 4]
   const void* bias;                    // [N] of the output's type, or null
   void* out;
   int64_t m, n, pitch, sa_pitch;       // pitch of out in elements; sa_pitch: m up to a multiple of 8
-  int kb;                              // Kp / 128
+  int kb, sb_pitch;                    // Kp / 128, and up to a multiple of 4
 };
 
 template <int I>
@@ -29,50 +31,6 @@ __device__ __forceinline__ void each(F& f) {
   if constexpr (I < N) {
     f(Index<I>{});
     each<N, I + 1>(f);
-  }
-}
-
-__device__ __forceinline__ i32x8 load32(const uint8_t* p) {
-  const i32x4 x = *(const i32x4*)p, y = *(const i32x4*)(p + 16);
-  return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
-template <bool POW2>
-__device__ __forceinline__ float scale_at(const void* s, int64_t at) {
-  if constexpr (POW2) {
-    const uint32_t b = ((const uint8_t*)s)[at];
-    return b == 255 ? __uint_as_float(0x7FC00000u) : b ? __uint_as_float(b << 23) : 5.877471754e-39f;
-  } else {
-    return ((const float*)s)[at];
-  }
-}
-
-// One wave a 16 x 16 tile. The weight is the matrix instruction's first operand, so that the four
-// sums of a lane are four neighbours n of one row m.
-template <typename O, bool POW2>
-__global__ __launch_bounds__(256) void k_simple(MatArgs p) {
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int64_t n0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16, m = (int64_t)blockIdx.y * 16 + c;
-  if (n0 >= p.n) return;
-  const int64_t kp = (int64_t)p.kb * kBlockK, bn = n0 + c < p.n ? n0 + c : p.n - 1, am = m < p.m ? m : p.m - 1;
-  const uint8_t *a = p.a + am * kp + g * 32, *b = p.b + bn * kp + g * 32;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int kb = 0; kb < p.kb; ++kb) {
-    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(load32(b + kb * kBlockK), load32(a + kb * kBlockK),
-                                                                    zero, 0, 0, 0, 0, 0, 0);
-    const float s = scale_at<POW2>(p.sa, (int64_t)kb * p.sa_pitch + am) * scale_at<POW2>(p.sb, n0 / kBlockK * p.kb + kb);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = fmaf(t[i], s, acc[i]);
-  }
-  if (m >= p.m) return;
-  using B = typename Bits<O>::type;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t n = n0 + g * 4 + i;
-    if (n >= p.n) continue;
-    const float v = acc[i] + (p.bias ? load_f32<O>(((const B*)p.bias)[n]) : 0.f);
-    ((B*)p.out)[m * p.pitch + n] = store_bits<O>(v);
   }
 }
 
@@ -90,16 +48,6 @@ __global__ __launch_bounds__(256) void k_simple(MatArgs p) {
 __host__ __device__ __forceinline__ constexpr int column_of(int piece, int c) {
   return (piece >> 1) * 32 + (c >> 2) * 8 + (piece & 1) * 4 + (c & 3);
 }
-
-template <int MT_, int NT_, int WM_, int WN_>
-struct Tile {
-  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_;
-  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
-  static constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN;
-  static constexpr int kBytes = (BM + BN) * kBlockK;              // one step of both tiles
-  static constexpr int kLoadsA = BM / 8 / kWaves, kLoadsB = BN / 8 / kWaves;   // 1024-byte loads of a wave
-  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "whole loads for every wave");
-};
 
 // Lane l's BYTES at base + voff + soff go to LDS at lds + BYTES * l. (m0 is the compiler's to set before its
 // own uses of it, and it makes none here.)
@@ -127,32 +75,12 @@ __device__ __forceinline__ u32x4 buffer_of(const void* base) {
   return r;
 }
 
-// Eight scales of a lane's rows m .. m + 7 of one block along K, as they are held. m is a multiple of 8 and
-// below the pitch, which is one too.
-template <bool POW2>
-struct Scales {
-  float f[POW2 ? 1 : 8];
-  uint32_t b[POW2 ? 2 : 1];
-  __device__ __forceinline__ void load(const void* base, int64_t at) {
-    if constexpr (POW2) {
-      const uint2 x = *(const uint2*)((const uint8_t*)base + at);
-      b[0] = x.x, b[1] = x.y;
-    } else {
-      const f32x4 *x = (const f32x4*)((const float*)base + at), u = x[0], v = x[1];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = u[i], f[4 + i] = v[i];
-    }
-  }
-  // The loads have arrived (and are not waited for again behind later ones).
-  __device__ __forceinline__ void arrived() {
-    if constexpr (POW2) {
-      asm volatile("" : "+v"(b[0]), "+v"(b[1]));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(f[i]));
-    }
-  }
-};
+// The buffer where there is something to load, and an empty one elsewhere: its loads are counted and waited for
+// like the others, and fetch nothing. So no load of a loop is behind a branch.
+__device__ __forceinline__ u32x4 if_any(u32x4 rsrc, bool any) {
+  rsrc[2] = __builtin_amdgcn_readfirstlane(any ? 0xFFFFFFFFu : 0u);
+  return rsrc;
+}
 
 __device__ __forceinline__ i32x8 join(const i32x4 (&v)[2]) {
   return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -176,45 +104,6 @@ __device__ __forceinline__ bool tile_of(int block, int tiles_m, int tiles_n, int
   tn = t % per / rows;
   return true;
 }
-
-// A wave's share of the loads of both tiles' steps into LDS. Rows past the end repeat the last one.
-template <typename T>
-struct Loader {
-  u32x4 ra, rb;
-  uint32_t va[T::kLoadsA], vb[T::kLoadsB], base;
-  int wave;
-  __device__ __forceinline__ Loader(const MatArgs& p, uint8_t* lds, int64_t m0, int64_t n0, int wave_, int lane)
-      : wave(wave_) {
-    const int64_t kp = (int64_t)p.kb * kBlockK;
-    base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    ra = buffer_of(p.a + m0 * kp);
-    rb = buffer_of(p.b + n0 * kp);
-#pragma unroll
-    for (int i = 0; i < T::kLoadsA; ++i) {
-      const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = row >> 1 & 7, piece = row >> 4;
-      const int64_t in = piece / T::MT * 16 * T::MT + (row & 15) * T::MT + piece % T::MT;
-      va[i] = (uint32_t)(min(in, p.m - 1 - m0) * kp + ((lane & 7) ^ key) * 16);
-    }
-#pragma unroll
-    for (int i = 0; i < T::kLoadsB; ++i) {
-      const int row = (wave + i * T::kWaves) * 8 + lane / 8, key = row >> 1 & 7, piece = row >> 4;
-      const int64_t in = piece / T::NT * 16 * T::NT + column_of(piece % T::NT, row & 15);
-      vb[i] = (uint32_t)(min(in, p.n - 1 - n0) * kp + ((lane & 7) ^ key) * 16);
-    }
-  }
-  // load i of the step's kLoadsA + kLoadsB
-  __device__ __forceinline__ void one(int i, int kb, int buf) {
-    const uint32_t to = base + buf * T::kBytes;
-    if (i < T::kLoadsA)
-      load_lds<16>(ra, va[i], kb * kBlockK, to + (wave + i * T::kWaves) * 1024);
-    else
-      load_lds<16>(rb, vb[i - T::kLoadsA], kb * kBlockK, to + T::BM * kBlockK + (wave + (i - T::kLoadsA) * T::kWaves) * 1024);
-  }
-  __device__ __forceinline__ void fetch(int kb, int buf) {
-#pragma unroll
-    for (int i = 0; i < T::kLoadsA + T::kLoadsB; ++i) one(i, kb, buf);
-  }
-};
 
 // A lane's MT rows from m on; n: the wave's first column.
 template <int MT, int NT, typename O>
@@ -256,87 +145,6 @@ __device__ __forceinline__ void store_tile(const MatArgs& p, const f32x4 (&acc)[
   }
 }
 
-template <typename T, typename O, bool POW2>
-__global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 2 : 1) void k_tile(MatArgs p, int tiles_m, int tiles_n) {
-  constexpr int MT = T::MT, NT = T::NT;
-  static_assert(MT == 8, "a lane's rows have one load of scales");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * T::kBytes];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4, wm = wave / T::WN, wn = wave % T::WN;
-
-  int tm, tn;
-  if (!tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn)) return;
-  const int64_t m0 = (int64_t)tm * T::BM, n0 = (int64_t)tn * T::BN;
-  Loader<T> loader(p, lds, m0, n0, wave, lane);
-
-  const int64_t m = m0 + wm * 16 * MT + c * MT, n = n0 + wn * 16 * NT;
-  const int64_t sa_at = min(m, p.sa_pitch - 8);       // rows past the end take scales of the last ones
-  const int64_t sb_at = min(n0 + wn * 16 * NT, p.n - 1) / kBlockK * p.kb;
-  Scales<POW2> sa;
-  float sb_f = 0.f;
-  uint32_t sb_b = 0;
-  auto scales = [&](int kb) {
-    sa.load(p.sa, kb * p.sa_pitch + sa_at);
-    if constexpr (POW2) sb_b = ((const uint8_t*)p.sb)[sb_at + kb];
-    else sb_f = ((const float*)p.sb)[sb_at + kb];
-  };
-
-  f32x4 acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const uint8_t* la = lds + (wm * 16 * MT + c) * kBlockK;
-  const uint8_t* lb = lds + T::BM * kBlockK + (wn * 16 * NT + c) * kBlockK;
-  const int piece0 = (g ^ (c >> 1)) * 16, piece1 = piece0 ^ 64;
-
-  loader.fetch(0, 0);
-  scales(0);
-  for (int kb = 0; kb < p.kb; ++kb) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    sa.arrived();
-    Scales<POW2> now = sa;
-    const float wf = sb_f;
-    const uint32_t wb = sb_b;
-    if (kb + 1 < p.kb) {
-      scales(kb + 1);
-      loader.fetch(kb + 1, (kb + 1) & 1);
-    }
-    const int buf = (kb & 1) * T::kBytes;
-    i32x8 w[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const i32x4 x = *(const i32x4*)(lb + buf + j * 16 * kBlockK + piece0);
-      const i32x4 y = *(const i32x4*)(lb + buf + j * 16 * kBlockK + piece1);
-      w[j] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-    auto row = [&](auto I) {
-      constexpr int i = decltype(I)::value;
-      const i32x4 x = *(const i32x4*)(la + buf + i * 16 * kBlockK + piece0);
-      const i32x4 y = *(const i32x4*)(la + buf + i * 16 * kBlockK + piece1);
-      const i32x8 v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        if constexpr (POW2) {
-          acc[i][j] = mfma_scaled<i & 3>(w[j], v, acc[i][j], wb, now.b[i >> 2]);
-        } else {
-          const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-          const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[j], v, zero, 0, 0, 0, 0, 0, 0);
-          const float s = now.f[i] * wf;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[r], s, acc[i][j][r]);
-        }
-      }
-    };
-    each<MT>(row);
-  }
-
-  store_tile<MT, NT, O>(p, acc, m, n, g);
-}
-
 // 256 x 256 for e8m0 scales with four waves of 128 x 128, one to a SIMD: the matrix instruction applies
 // the scales, so the sums never leave the accumulation registers, and fewer bytes leave LDS than with
 // eight waves of 128 x 64 (128 KB a step instead of 192 KB, at 128 B a cycle and 2048 cycles of products).
@@ -352,9 +160,9 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 2 : 1) void k_til
 // A load has six quarters (3072 cycles) to arrive; every wave counts its own loads (4, 4, 4 and 5 a quarter)
 // and waits for those that the quarter reads, and the barrier joins the waits of all four. What a
 // quarter loads into was read a step before (x0: waited for by count at Q0; the others: their
-// products have been issued). The last steps load their last tile again, which nobody reads.
+// products have been issued).
 struct Quarters {
-  static constexpr int BM = 256, BN = 256, kThreads = 256;
+  static constexpr int BM = 256, BN = 256;
   static constexpr int kPart = 128 * kBlockK;                     // x0, x1, w0 or w1 of one step: 16 KB
   static constexpr int kStep = 4 * kPart, kScales = 2 * kStep;    // then 4 steps x 4 waves x 256 scales
   static constexpr int kLds = kScales + 4 * 4 * 256;
@@ -398,16 +206,16 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
     }
   const uint32_t vs = (uint32_t)min((int64_t)lane * 4, p.sa_pitch - 4 - m0);
   auto load_x = [&](int part, int i, int k) {
-    load_lds<16>(rx, vx[part * 4 + i], min(k, last) * kBlockK,
+    load_lds<16>(if_any(rx, k <= last), vx[part * 4 + i], k * kBlockK,
                  base + (k & 1) * Q::kStep + part * Q::kPart + (wave + 4 * i) * 1024);
   };
   auto load_w = [&](int part, int i, int k) {
-    load_lds<16>(rw, vw[part * 4 + i], min(k, last) * kBlockK,
+    load_lds<16>(if_any(rw, k <= last), vw[part * 4 + i], k * kBlockK,
                  base + (k & 1) * Q::kStep + (2 + part) * Q::kPart + (wave + 4 * i) * 1024);
   };
   auto load_s = [&](int k) {
-    const u32x4 rs = buffer_of((const uint8_t*)p.sa + m0 + min(k, last) * p.sa_pitch);
-    load_lds<4>(rs, vs, 0, base + Q::kScales + ((k & 3) * 4 + wave) * 256);
+    const u32x4 rs = buffer_of((const uint8_t*)p.sa + m0 + k * p.sa_pitch);
+    load_lds<4>(if_any(rs, k <= last), vs, 0, base + Q::kScales + ((k & 3) * 4 + wave) * 256);
   };
 
   const int piece = (g ^ (c >> 1)) * 16;
@@ -423,13 +231,8 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
   };
 
   // the columns' scales of 256 steps: four in each lane
-  const uint8_t* sb = (const uint8_t*)p.sb + min(n0 + wn * 128, p.n - 1) / kBlockK * p.kb;
-  auto column_scales = [&](int k) {
-    uint32_t v = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v |= (uint32_t)sb[min(k + lane * 4 + i, last)] << (8 * i);
-    return v;
-  };
+  const uint8_t* sb = (const uint8_t*)p.sb + min(n0 + wn * 128, p.n - 1) / kBlockK * p.sb_pitch;
+  auto column_scales = [&](int k) { return ((const uint32_t*)sb)[min((k >> 2) + lane, last >> 2)]; };
   uint32_t sbs = column_scales(0);
   asm volatile("" : "+v"(sbs));
 
@@ -522,7 +325,7 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
 //   after the second          rows' pieces 4-7 (k+2), rows' scales (k+3)
 // so a load has a step and a half to arrive. Each wave counts its own loads: 6 and 3.
 struct Eight {
-  static constexpr int BM = 256, BN = 256, kThreads = 512;
+  static constexpr int BM = 256, BN = 256;
   static constexpr int kRows = 128 * kBlockK;                     // half of the rows' pieces: 16 KB
   static constexpr int kStep = 4 * kRows, kScales = 2 * kStep;    // then 4 steps x 256 scales
   static constexpr int kLds = kScales + 4 * 1024;
@@ -557,16 +360,16 @@ __global__ __launch_bounds__(512, 2) void k_eight(MatArgs p, int tiles_m, int ti
     vw[i] = (uint32_t)(min(at, p.n - 1 - n0) * kp + ((lane & 7) ^ (row >> 1 & 7)) * 16);
   }
   auto load_x = [&](int half, int i, int k) {
-    load_lds<16>(rx, vx[half * 2 + i], min(k, last) * kBlockK,
+    load_lds<16>(if_any(rx, k <= last), vx[half * 2 + i], k * kBlockK,
                  base + (k & 1) * Q::kStep + half * Q::kRows + (wave + 8 * i) * 1024);
   };
   auto load_w = [&](int i, int k) {
-    load_lds<16>(rw, vw[i], min(k, last) * kBlockK, base + (k & 1) * Q::kStep + 2 * Q::kRows + (wave + 8 * i) * 1024);
+    load_lds<16>(if_any(rw, k <= last), vw[i], k * kBlockK, base + (k & 1) * Q::kStep + 2 * Q::kRows + (wave + 8 * i) * 1024);
   };
   const uint32_t vs = (uint32_t)min((int64_t)(wave & 3) * 64 + lane, p.sa_pitch - 1 - m0) * 4;
   auto load_s = [&](int k) {                                      // waves 4-7 write the same once more
-    const u32x4 rs = buffer_of((const float*)p.sa + m0 + min(k, last) * p.sa_pitch);
-    load_lds<4>(rs, vs, 0, base + Q::kScales + (k & 3) * 1024 + (wave & 3) * 256);
+    const u32x4 rs = buffer_of((const float*)p.sa + m0 + k * p.sa_pitch);
+    load_lds<4>(if_any(rs, k <= last), vs, 0, base + Q::kScales + (k & 3) * 1024 + (wave & 3) * 256);
   };
 
   const int piece = (g ^ (c >> 1)) * 16;
@@ -582,7 +385,7 @@ __global__ __launch_bounds__(512, 2) void k_eight(MatArgs p, int tiles_m, int ti
   };
 
   // the columns' scales of 64 steps: one in each lane
-  const float* sb = (const float*)p.sb + min(n, p.n - 1) / kBlockK * p.kb;
+  const float* sb = (const float*)p.sb + min(n, p.n - 1) / kBlockK * p.sb_pitch;
   float sbs = sb[min(lane, last)];
   asm volatile("" : "+v"(sbs));
 
@@ -658,18 +461,6 @@ __global__ __launch_bounds__(512, 2) void k_eight(MatArgs p, int tiles_m, int ti
   store_tile<8, 4, O>(p, acc, m, n, g);
 }
 
-template <typename T, typename O>
-int run_tile(const MatArgs& p, bool pow2, hipStream_t s) {
-  const int64_t tm = (p.m + T::BM - 1) / T::BM, tn = (p.n + T::BN - 1) / T::BN, total = tm * tn;
-  if (total > (1 << 30)) return -1;
-  const unsigned grid = (unsigned)((total + 7) / 8 * 8);
-  if (pow2) k_tile<T, O, true><<<grid, T::kThreads, 0, s>>>(p, (int)tm, (int)tn);
-  else k_tile<T, O, false><<<grid, T::kThreads, 0, s>>>(p, (int)tm, (int)tn);
-  return (int)hipGetLastError();
-}
-
-using Big = Tile<8, 4, 2, 4>;
-
 template <typename O>
 int run_256(const MatArgs& p, bool pow2, hipStream_t s) {
   const int64_t tm = (p.m + 255) / 256, tn = (p.n + 255) / 256, total = tm * tn;
@@ -705,23 +496,26 @@ __device__ __forceinline__ void store4(const MatArgs& p, f32x4 v, int64_t m, int
 // K in gridDim.y parts whose float32 sums go to a workspace and are joined by k_join in the order of the parts. With two
 // stages (66 KB) two workgroups share a CU and run while the other waits; with four, one has three steps of loads in flight.
 struct Mid {
-  static constexpr int BM = 128, BN = 128, kThreads = 256;
+  static constexpr int BM = 128, BN = 128;
   static constexpr int kTile = 128 * kBlockK;                     // rows' or columns' step: 16 KB
   static constexpr int kStage = 2 * kTile + 4 * 256;              // and each wave's rows' scales
   static constexpr int kLoads = 9;                                // of a wave and step
 };
 
+// (LDS is given at the launch: with its size in the kernel the compiler would reckon with one workgroup on a CU for four
+// stages, spread the sums over the accumulation registers and move them to and fro every step.)
 template <int STAGES, typename O, bool POW2>
-__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void k_mid(MatArgs p, int tiles_m, int tiles_n, float* parts) {
+__global__ __launch_bounds__(256, 2) void k_mid(MatArgs p, int tiles_m, int tiles_n, float* parts) {
   using Q = Mid;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * Q::kStage];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
   int tm, tn;
   if (!tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn)) return;
   const int64_t m0 = (int64_t)tm * Q::BM, n0 = (int64_t)tn * Q::BN, kp = (int64_t)p.kb * kBlockK;
   const int64_t m = m0 + wm * 64 + c * 4, n = n0 + wn * 64;
-  const int first = (int)((int64_t)p.kb * blockIdx.y / gridDim.y), end = (int)((int64_t)p.kb * (blockIdx.y + 1) / gridDim.y);
+  const int first = __builtin_amdgcn_readfirstlane((uint32_t)p.kb * blockIdx.y / gridDim.y);
+  const int end = __builtin_amdgcn_readfirstlane((uint32_t)p.kb * (blockIdx.y + 1) / gridDim.y);
 
   const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   const u32x4 rx = buffer_of(p.a + m0 * kp), rw = buffer_of(p.b + n0 * kp);
@@ -739,11 +533,11 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void k_mid(MatArgs p, int
   auto fetch = [&](int k, int stage) {
     const uint32_t to = base + stage * Q::kStage;
     const u32x4 rs = buffer_of((const uint8_t*)p.sa + (m0 + k * p.sa_pitch) * kScale);
-    load_lds<4>(rs, vs, 0, to + 2 * Q::kTile + wave * 256);
+    load_lds<4>(if_any(rs, k < end), vs, 0, to + 2 * Q::kTile + wave * 256);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_lds<16>(rx, vx[i], k * kBlockK, to + (wave + 4 * i) * 1024);
+    for (int i = 0; i < 4; ++i) load_lds<16>(if_any(rx, k < end), vx[i], k * kBlockK, to + (wave + 4 * i) * 1024);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_lds<16>(rw, vw[i], k * kBlockK, to + Q::kTile + (wave + 4 * i) * 1024);
+    for (int i = 0; i < 4; ++i) load_lds<16>(if_any(rw, k < end), vw[i], k * kBlockK, to + Q::kTile + (wave + 4 * i) * 1024);
   };
 
   const int piece = (g ^ (c >> 1)) * 16;
@@ -751,21 +545,10 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void k_mid(MatArgs p, int
   const uint8_t* lw = lds + Q::kTile + (wn * 64 + c) * kBlockK;
   const uint8_t* ls = lds + 2 * Q::kTile + wave * 256 + (POW2 ? wm * 64 + c * 4 : c * 16);
 
-  // the columns' scales: of 256 steps, four bytes in a lane, or of 64, a float in a lane
-  constexpr int kChunk = POW2 ? 256 : 64;
-  const int64_t sb_at = min(n, p.n - 1) / kBlockK * p.kb;
-  auto column_scales = [&](int k) {
-    uint32_t v = 0;
-    if constexpr (POW2) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v |= (uint32_t)((const uint8_t*)p.sb)[sb_at + min(k + lane * 4 + i, end - 1)] << (8 * i);
-    } else {
-      v = ((const uint32_t*)p.sb)[sb_at + min(k + lane, end - 1)];
-    }
-    asm volatile("" : "+v"(v));
-    return v;
-  };
-  uint32_t sbs = column_scales(first);
+  // the columns' scale of a step, by scalar loads (address space 4): four bytes, or a float
+  typedef const uint32_t __attribute__((address_space(4))) * Scalars;
+  const Scalars sb = (Scalars)((const uint8_t*)p.sb + min(n, p.n - 1) / kBlockK * p.sb_pitch * kScale);
+  auto column_scale = [&](int k) { return POW2 ? sb[k >> 2] >> (8 * (k & 3)) : sb[k]; };
 
   f32x4 acc[4][4];
 #pragma unroll
@@ -774,104 +557,119 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void k_mid(MatArgs p, int
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
 #pragma unroll
-  for (int d = 0; d < STAGES - 1; ++d)
-    if (first + d < end) fetch(first + d, d);
-  int stage = 0;
-#pragma unroll 1
-  for (int k = first; k < end; ++k) {
-    const int done = k - first;
-    if (done && done % kChunk == 0) sbs = column_scales(k);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the last step's reads
-    if (k + STAGES - 2 < end) meet<(STAGES - 2) * Q::kLoads>();
-    else meet<0>();
-    if (k + STAGES - 1 < end) fetch(k + STAGES - 1, stage ? stage - 1 : STAGES - 1);
-    const int at = stage * Q::kStage;
+  for (int d = 0; d < STAGES; ++d) fetch(first + d, d);
+  // operands of two steps: one in use, one being read
+  struct Step {
     i32x4 x[4][2], w[4][2];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        w[j][h] = *(const i32x4*)(lw + at + j * 16 * kBlockK + (h ? piece ^ 64 : piece));
-        x[j][h] = *(const i32x4*)(lx + at + j * 16 * kBlockK + (h ? piece ^ 64 : piece));
-      }
-    uint32_t xb = 0, wb = 0;
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (POW2) {
-      xb = *(const uint32_t*)(ls + at);
-      wb = __builtin_amdgcn_readlane(sbs, done >> 2 & 63) >> (8 * (done & 3));
+    f32x4 s;
+    uint32_t b, c;
+  } step[2];
+  // read number `at` of 17: a step's first products need its first columns and all its rows
+  auto read = [&](Step& to, int from, int at) {
+    const int i = at / 2 % 4, h = at & 1, row = i * 16 * kBlockK + (h ? piece ^ 64 : piece);
+    if (at == 16) {
+      if constexpr (POW2) to.b = *(const uint32_t*)(ls + from);
+      else to.s = *(const f32x4*)(ls + from);
+    } else if (at < 8) {
+      to.x[i][h] = *(const i32x4*)(lx + from + row);
     } else {
-      s = *(const f32x4*)(ls + at) * __uint_as_float(__builtin_amdgcn_readlane(sbs, done & 63));
+      to.w[i][h] = *(const i32x4*)(lw + from + row);
     }
-    auto row = [&](auto I) {
-      constexpr int i = decltype(I)::value;
+  };
+  meet<(STAGES - 1) * Q::kLoads>();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (POW2) {
-          acc[i][j] = mfma_scaled<i>(join(w[j]), join(x[i]), acc[i][j], wb, xb);
-        } else {
-          const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-          const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(w[j]), join(x[i]), zero, 0, 0, 0, 0, 0, 0);
+  for (int at = 0; at < 17; ++at) read(step[0], 0, at);
+  step[0].c = column_scale(first);
+
+  int stage = 0;                                // step k's
+  auto one_step = [&](int k, const Step& now, Step& next) {
+    // step k is in this wave's registers, and after the meeting in every wave's; step k + 1 is in LDS
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    meet<(STAGES - 2) * Q::kLoads>();
+    const int ahead = stage + 1 < STAGES ? stage + 1 : 0, from = ahead * Q::kStage;
+    fetch(k + STAGES, stage);
+    stage = ahead;
+    next.c = column_scale(min(k + 1, end - 1));
+    f32x4 t[4], s;
+    if constexpr (!POW2) s = now.s * __uint_as_float(now.c);
+    auto add = [&](auto At) {
+      constexpr int at = decltype(At)::value, j = at / 4, i = at % 4;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[r], s[i], acc[i][j][r]);
-        }
-      }
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[i][r], s[i], acc[i][j][r]);
     };
-    each<4>(row);
-    stage = stage + 1 < STAGES ? stage + 1 : 0;
+    auto one = [&](auto At) {
+      constexpr int at = decltype(At)::value, j = at / 4, i = at % 4;
+      if constexpr (POW2) {
+        acc[i][j] = mfma_scaled<i>(join(now.w[j]), join(now.x[i]), acc[i][j], now.c, now.b);
+      } else {
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        t[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(now.w[j]), join(now.x[i]), zero, 0, 0, 0, 0, 0, 0);
+        if constexpr (at >= 2) add(Index<at - 2>{});
+      }
+      read(next, from, at);
+      if (at == 15) read(next, from, 16);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    each<16>(one);
+    if constexpr (!POW2) {
+      add(Index<14>{});
+      add(Index<15>{});
+    }
+  };
+#pragma unroll 1
+  for (int k = first; k + 1 < end; k += 2) {
+    one_step(k, step[0], step[1]);
+    one_step(k + 1, step[1], step[0]);
   }
+  if ((end - first) & 1) one_step(end - 1, step[0], step[1]);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing may reach LDS after the workgroup's end
   if (!parts) {
     store_tile<4, 4, O>(p, acc, m, n, g);
     return;
   }
-  // this part's sums, float32, rows of n up to a multiple of 4
-  const int64_t wide = (p.n + 3) / 4 * 4;
-  float* out = parts + ((int64_t)blockIdx.y * p.m + m) * wide;
+  // this part's sums as they lie in the registers: each store a whole KB
+  f32x4* out = (f32x4*)parts + (((int64_t)blockIdx.y * tiles_m * tiles_n + (int64_t)tm * tiles_n + tn) * 4 + wave) * 1024 + lane;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (m + i >= p.m) break;
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t at = n + g * 8 + (j >> 1) * 32 + (j & 1) * 4;
-      if (at < p.n) *(f32x4*)(out + i * wide + at) = acc[i][j];
-    }
-  }
+    for (int j = 0; j < 4; ++j) out[(i * 4 + j) * 64] = acc[i][j];
 }
 
-// out = the sum of the parts in their order, plus bias: four neighbours a lane.
+// out = the sum of the parts in their order, plus bias: four neighbours a lane, a tile every 16 workgroups.
 template <typename O>
-__global__ __launch_bounds__(256) void k_join(MatArgs p, const float* parts, int count) {
-  const int64_t quads = (p.n + 3) / 4, m = blockIdx.y, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= quads) return;
-  const f32x4* in = (const f32x4*)parts + m * quads + at;
+__global__ __launch_bounds__(256) void k_join(MatArgs p, int tiles_m, int tiles_n, const f32x4* parts, int count) {
+  const int tile = blockIdx.x / 16, at = blockIdx.x % 16 * 256 + threadIdx.x;
+  const int wave = at >> 10, i = at >> 8 & 3, j = at >> 6 & 3, c = at & 15, g = at >> 4 & 3;
+  const int64_t m = (int64_t)(tile / tiles_n) * 128 + (wave >> 1) * 64 + c * 4 + i;
+  const int64_t n = (int64_t)(tile % tiles_n) * 128 + (wave & 1) * 64 + (j >> 1) * 32 + g * 8 + (j & 1) * 4;
+  if (m >= p.m || n >= p.n) return;
+  const f32x4* in = parts + (int64_t)tile * 4096 + at;
+  const int64_t apart = (int64_t)tiles_m * tiles_n * 4096;
   f32x4 v = in[0];
-  for (int i = 1; i < count; ++i) v += in[i * p.m * quads];
-  store4<O>(p, v, m, at * 4);
+  for (int k = 1; k < count; ++k) v += in[k * apart];
+  store4<O>(p, v, m, n);
 }
 
 template <typename O>
 int run_mid(const MatArgs& p, bool pow2, int count, float* parts, hipStream_t s) {
   const int64_t tm = (p.m + 127) / 128, tn = (p.n + 127) / 128, total = tm * tn;
-  if (total > (1 << 30) || count > 65535) return -1;
+  if (total > (1 << 26) || count > 65535) return -1;
   const dim3 grid((unsigned)((total + 7) / 8 * 8), count);
   float* to = count > 1 ? parts : nullptr;
   if (total * count > 256) {
-    if (pow2) k_mid<2, O, true><<<grid, 256, 0, s>>>(p, (int)tm, (int)tn, to);
-    else k_mid<2, O, false><<<grid, 256, 0, s>>>(p, (int)tm, (int)tn, to);
+    if (pow2) k_mid<2, O, true><<<grid, 256, 2 * Mid::kStage, s>>>(p, (int)tm, (int)tn, to);
+    else k_mid<2, O, false><<<grid, 256, 2 * Mid::kStage, s>>>(p, (int)tm, (int)tn, to);
   } else {
-    if (pow2) k_mid<4, O, true><<<grid, 256, 0, s>>>(p, (int)tm, (int)tn, to);
-    else k_mid<4, O, false><<<grid, 256, 0, s>>>(p, (int)tm, (int)tn, to);
+    if (pow2) k_mid<4, O, true><<<grid, 256, 4 * Mid::kStage, s>>>(p, (int)tm, (int)tn, to);
+    else k_mid<4, O, false><<<grid, 256, 4 * Mid::kStage, s>>>(p, (int)tm, (int)tn, to);
   }
-  if (count > 1) {
-    const int64_t gx = ((p.n + 3) / 4 + 255) / 256;
-    if (gx > 0x7FFFFFFF || p.m > 65535) return -1;
-    k_join<O><<<dim3((unsigned)gx, (unsigned)p.m), 256, 0, s>>>(p, parts, count);
-  }
+  if (count > 1) k_join<O><<<(unsigned)(total * 16), 256, 0, s>>>(p, (int)tm, (int)tn, (const f32x4*)parts, count);
   return (int)hipGetLastError();
 }
 
 // ---------------------------------------------------------------- few rows
 //
-// Up to 128 rows the weight's bytes are what counts: one workgroup takes all rows and 16 * NP columns, its waves
+// Up to 64 rows the weight's bytes are what counts: one workgroup takes all rows and 16 * NP columns, its waves
 // take every WAVES-th block of K and read their operands from memory straight into registers, DEPTH
 // blocks ahead, each weight byte once on the whole card; the rows are read again by each workgroup, out of L2.
 // No wave waits for another until the end, when the waves' sums are added through LDS in the order of
@@ -887,7 +685,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_narrow(MatArgs p) {
   for (int i = 0; i < MP; ++i) px[i] = p.a + min((int64_t)c * MP + i, p.m - 1) * kp + g * 16;
 #pragma unroll
   for (int j = 0; j < NP; ++j) pw[j] = p.b + min(n0 + (NP == 2 ? column_of(j, c) : c), p.n - 1) * kp + g * 16;
-  const int64_t sa_at = min((int64_t)c * MP, p.sa_pitch - MP), sb_at = n0 / kBlockK * p.kb;
+  const int64_t sa_at = min((int64_t)c * MP, p.sa_pitch - MP), sb_at = n0 / kBlockK * p.sb_pitch;
 
   struct Block {
     i32x4 x[MP][2], w[NP][2];
@@ -999,23 +797,53 @@ int narrow(const MatArgs& p, bool pow2, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
-template <typename O>
-int run_simple(const MatArgs& p, bool pow2, hipStream_t s) {
-  const int64_t gx = (p.n + 63) / 64, gy = (p.m + 15) / 16;
-  if (gx > 0x7FFFFFFF || gy > 65535) return -1;
-  const dim3 grid((unsigned)gx, (unsigned)gy);
-  if (pow2) k_simple<O, true><<<grid, 256, 0, s>>>(p);
-  else k_simple<O, false><<<grid, 256, 0, s>>>(p);
-  return (int)hipGetLastError();
+// ---------------------------------------------------------------- which one
+//
+// By sizes alone, the least of these estimates (us; what the kernels took on an MI355X, sums to 5 TB/s):
+//   few rows    2 + (weight + rows for every 32 columns) / 8 MB           (64 x 8192 x 8192: 24)
+//   128 x 128   5.5 + steps * (0.47, or 0.95 a round of 512 workgroups, float scales 1.1)
+//               + 3 + twice the parts' bytes / 5 MB where K has parts     (777 x 5000 x 1928: 17, 27 with 256 x 256;
+//                                                                          128 x 8192 x 4096 in 2 parts 17, in 1 21)
+//   256 x 256   rounds of 256 * (8 + steps * (1.45, float scales 1.6)),   (4096 x 4096 x 4096: 55, 65 with 128 x 128;
+//               a last round of a share f of them counts (1 + f) / 2       4096 x 10240 x 4096: 163, 194 with 128 x 128)
+struct Plan {
+  enum { kNarrow, kMid, k256 } kind;
+  int parts;
+  int64_t bytes;                        // of workspace
+};
+
+Plan plan(int64_t m, int64_t n, int kb, bool pow2) {
+  const double weight = (double)n * kb * kBlockK;
+  Plan best = {Plan::k256, 1, 0};
+  const int64_t big = (m + 255) / 256 * ((n + 255) / 256), tiles = (m + 127) / 128 * ((n + 127) / 128);
+  const double rest = big % 256 ? (1 + big % 256 / 256.0) / 2 : 0;
+  double least = (std::max<double>(big / 256 + rest, 1)) * (8 + kb * (pow2 ? 1.45 : 1.6));
+  if (m <= 64) {
+    const int rows = m <= 16 ? 16 : m <= 32 ? 32 : 64;
+    const double t = 2 + weight * (1 + rows / 32.0) / 8e6;
+    if (t < least) least = t, best = {Plan::kNarrow, 1, 0};
+  }
+  for (int parts = 1; parts <= 16 && parts * 2 <= kb; parts *= 2) {
+    if (parts > 1 && tiles * parts > 512) break;
+    const int64_t bytes = parts > 1 ? tiles * parts * 128 * 128 * 4 : 0;
+    const int steps = (kb + parts - 1) / parts;
+    const double step = tiles * parts <= 256 ? 0.47 : (double)((tiles * parts + 511) / 512) * (pow2 ? 0.95 : 1.1);
+    const double t = 5.5 + steps * step + (parts > 1 ? 3 + 2 * bytes / 5e6 : 0);
+    if (t < least) least = t, best = {Plan::kMid, parts, bytes};
+  }
+  return best;
 }
 
 template <typename O>
-int run(const MatArgs& p, bool pow2, hipStream_t s) {
-  if (p.m > 128) return run_256<O>(p, pow2, s);
+int run(const MatArgs& p, bool pow2, float* workspace, int64_t bytes, hipStream_t s) {
+  const Plan to = plan(p.m, p.n, p.kb, pow2);
+  if (to.bytes > bytes || (to.bytes && !workspace)) return -1;
+  if (to.kind == Plan::k256) return run_256<O>(p, pow2, s);
+  if (to.kind == Plan::kMid) return run_mid<O>(p, pow2, to.parts, workspace, s);
+  // two pieces of columns a workgroup halve what is read of the rows, where that leaves enough workgroups
   if (p.m <= 16) return p.n >= 8192 ? narrow<1, 2, 8, 4, O>(p, pow2, s) : narrow<1, 1, 8, 4, O>(p, pow2, s);
-  if (p.m <= 32) return p.n >= 8192 ? narrow<2, 2, 8, 4, O>(p, pow2, s) : narrow<2, 1, 8, 4, O>(p, pow2, s);
-  if (p.m <= 64) return narrow<4, 2, 8, 3, O>(p, pow2, s);
-  return narrow<8, 2, 8, 2, O>(p, pow2, s);
+  if (p.m <= 32) return narrow<2, 2, 8, 4, O>(p, pow2, s);
+  return narrow<4, 2, 8, 2, O>(p, pow2, s);
 }
 
 }  // namespace
@@ -1025,20 +853,29 @@ using namespace yoda_fp8;
 
 extern "C" {
 
+// Bytes of workspace that a product of these sizes needs (16-byte aligned, its own for the length of the call).
+int64_t yoda_fp8_matmul_workspace(int64_t m, int64_t n, int kb, int pow2) {
+  return m < 1 || n < 1 || kb < 1 ? 0 : plan(m, n, kb, pow2).bytes;
+}
+
 // kb: blocks along K. pitch: elements between rows of out. sa_pitch: scales between a's blocks along K,
-// a multiple of 8, the scales 16-byte aligned. Returns 0, a hipError, or -1 for
-// arguments out of range.
+// a multiple of 8. Rows of values and scales are 16-byte aligned. Returns 0, a hipError, or -1 for arguments
+// out of range.
 int yoda_fp8_matmul(int device, void* stream, int out_type, int pow2, const void* a, const void* sa, const void* b,
-                    const void* sb, const void* bias, void* out, int64_t m, int64_t n, int kb, int64_t pitch, int64_t sa_pitch) {
-  if ((out_type != kBf16 && out_type != kFp16) || m < 0 || n < 0 || kb < 1 || kb > 65535 || pitch < n || sa_pitch < m || sa_pitch % 8) return -1;
+                    const void* sb, const void* bias, void* out, int64_t m, int64_t n, int kb, int64_t pitch,
+                    int64_t sa_pitch, void* workspace, int64_t workspace_bytes) {
+  if ((out_type != kBf16 && out_type != kFp16) || m < 0 || n < 0 || kb < 1 || kb > 65535 || pitch < n || sa_pitch < m ||
+      sa_pitch % 8)
+    return -1;
   if (m == 0 || n == 0) return 0;
   if (!a || !sa || !b || !sb || !out) return -1;
   DeviceScope on(device);
   if (on.err != hipSuccess) return (int)on.err;
-  const MatArgs p = {(const uint8_t*)a, (const uint8_t*)b, sa, sb, bias, out, m, n, pitch, sa_pitch, kb};
+  const MatArgs p = {(const uint8_t*)a, (const uint8_t*)b, sa, sb, bias, out, m, n, pitch, sa_pitch, kb, (kb + 3) / 4 * 4};
   const hipStream_t s = (hipStream_t)stream;
-  if (out_type == kFp16) return run<__half>(p, pow2, s);
-  return run<__hip_bfloat16>(p, pow2, s);
+  float* ws = (float*)workspace;
+  if (out_type == kFp16) return run<__half>(p, pow2, ws, workspace_bytes, s);
+  return run<__hip_bfloat16>(p, pow2, ws, workspace_bytes, s);
 }
 
 }  // extern "C"

@@ -19,6 +19,7 @@ that requires a gradient is refused while gradients are recorded.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -43,15 +44,26 @@ def _lib() -> tuple:
     return _fns
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace(m: int, n: int, kb: int, pow2: bool) -> int:
+    """Bytes of workspace that the product of these sizes asks for."""
+    return hip.lib().yoda_fp8_matmul_workspace(m, n, kb, pow2)
+
+
 def blocks(n: int) -> int:
     """Blocks of 128 that cover ``n``."""
     return -(-n // BLOCK)
 
 
-def _row_scales(rows: int, kb: int, dtype: torch.dtype, device, zeros: bool = False) -> torch.Tensor:
-    """[rows, kb] scales of 1 x 128 blocks: kb runs of ``rows``, a multiple of 8 apart."""
-    make = torch.zeros if zeros else torch.empty
-    return make((kb, -(-rows // 8) * 8), dtype=dtype, device=device)[:, :rows].t()
+def _scales(rows: int, kb: int, block_rows: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """Room for the scales of ``rows`` (of blocks) x ``kb`` blocks, in the kernels' layout."""
+    if block_rows == 1:
+        pitch = -(-rows // 8) * 8
+        s = torch.empty_strided((pitch, kb), (1, pitch), dtype=dtype, device=device)
+        return s if pitch == rows else s[:rows]
+    pitch = -(-kb // 4) * 4
+    s = torch.empty((rows, pitch), dtype=dtype, device=device)
+    return s if pitch == kb else s[:, :kb]
 
 
 class BlockMatrix:
@@ -59,7 +71,8 @@ class BlockMatrix:
 
     ``data``    [rows, 128 · blocks(cols)] e4m3, contiguous; the columns from ``cols`` on are zero
     ``scales``  [blocks of rows, blocks of columns], float32 or e8m0. For ``block_rows`` 1 they lie
-                block by block, each block's rows padded to a multiple of 8, for 128 row by row.
+                block by block, each block's rows padded to a multiple of 8, for 128 row by row, each
+                row padded to a multiple of 4.
 
     The constructor takes values that exist already (a checkpoint's): unpadded ones and scales in
     the other order are laid out once, here. Padded ones must hold zeros from ``cols`` on.
@@ -93,12 +106,10 @@ class BlockMatrix:
             values = values.contiguous()
         if values.data_ptr() % 16:
             values = values.clone()
-        if block_rows == 1:
-            pitch = -(-rows // 8) * 8
-            if scales.stride() != (1, pitch) or scales.data_ptr() % 16:
-                scales = _row_scales(rows, kb, scales.dtype, scales.device, zeros=True).copy_(scales)
-        elif not scales.is_contiguous():
-            scales = scales.contiguous()
+        stride = (1, -(-rows // 8) * 8) if block_rows == 1 else (-(-kb // 4) * 4, 1)
+        # (a view that has the strides by chance may end before its padding)
+        if scales.stride() != stride or scales.data_ptr() % 16 or (rows % 8 if block_rows == 1 else kb % 4):
+            scales = _scales(*want, block_rows, scales.dtype, scales.device).copy_(scales)
         self.data, self.scales, self.rows, self.cols, self.block_rows = values, scales, rows, cols, block_rows
 
     @classmethod
@@ -106,10 +117,7 @@ class BlockMatrix:
         m = cls.__new__(cls)
         kb = blocks(cols)
         m.data = torch.empty((rows, kb * BLOCK), dtype=E4M3, device=device)
-        if block_rows == 1:
-            m.scales = _row_scales(rows, kb, scale_dtype, device)
-        else:
-            m.scales = torch.empty((blocks(rows), kb), dtype=scale_dtype, device=device)
+        m.scales = _scales(rows if block_rows == 1 else blocks(rows), kb, block_rows, scale_dtype, device)
         m.rows, m.cols, m.block_rows = rows, cols, block_rows
         return m
 
@@ -249,8 +257,11 @@ def matmul(a: BlockMatrix, b: BlockMatrix, out_dtype: torch.dtype = torch.bfloat
             raise ValueError(f"out: {(m, n)} on {device} with rows apart, not {tuple(out.shape)} on {out.device} "
                              f"with strides {out.stride()}")
         _no_grad(out)
-    _ok(_lib()[2](device.index, _stream(device), _OUT[out_dtype], a.scales.dtype is E8M0, a.data.data_ptr(),
-                  a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(),
-                  None if bias is None else bias.data_ptr(), out.data_ptr(), m, n, blocks(a.cols),
-                  max(out.stride(0), n), -(-m // 8) * 8), "fp8 matmul")
+    kb, pow2 = blocks(a.cols), a.scales.dtype is E8M0
+    room = _workspace(m, n, kb, pow2)
+    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+    _ok(_lib()[2](device.index, _stream(device), _OUT[out_dtype], pow2, a.data.data_ptr(), a.scales.data_ptr(),
+                  b.data.data_ptr(), b.scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(),
+                  m, n, kb, max(out.stride(0), n), -(-m // 8) * 8, None if ws is None else ws.data_ptr(), room),
+        "fp8 matmul")
     return out

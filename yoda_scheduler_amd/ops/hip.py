@@ -49,7 +49,8 @@ def _declare(lib: ctypes.CDLL) -> None:
         "yoda_fp8_quantize": [c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
                               c_int],
         "yoda_fp8_matmul": [c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                            c_int64, c_int64, c_int, c_int64, c_int64],
+                            c_int64, c_int64, c_int, c_int64, c_int64, c_void_p, c_int64],
+        "yoda_fp8_matmul_workspace": [c_int64, c_int64, c_int, c_int],
     }
     for name, args in sigs.items():
         f = getattr(lib, name, None)
@@ -58,7 +59,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         if f is None:
             raise AttributeError(f"{PATH} has no {name}")
         f.argtypes = args
-        f.restype = c_int
+        f.restype = c_int64 if name.endswith("_workspace") else c_int
     try:
         from . import device_scorer as _ds
     except ImportError:
