@@ -55,15 +55,12 @@ def blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
-def _scales(rows: int, kb: int, block_rows: int, dtype: torch.dtype, device) -> torch.Tensor:
-    """Room for the scales of ``rows`` (of blocks) x ``kb`` blocks, in the kernels' layout."""
+def _scales(like: torch.Tensor, rows: int, kb: int, block_rows: int, dtype: torch.dtype) -> torch.Tensor:
+    """Room for the scales of ``rows`` (of blocks) x ``kb`` blocks and their padding, in the kernels' layout."""
     if block_rows == 1:
-        pitch = -(-rows // 8) * 8
-        s = torch.empty_strided((pitch, kb), (1, pitch), dtype=dtype, device=device)
-        return s if pitch == rows else s[:rows]
-    pitch = -(-kb // 4) * 4
-    s = torch.empty((rows, pitch), dtype=dtype, device=device)
-    return s if pitch == kb else s[:, :kb]
+        pitch = (rows + 7) // 8 * 8
+        return torch.empty_strided((pitch, kb), (1, pitch), dtype=dtype, device=like.device)
+    return like.new_empty((rows, (kb + 3) // 4 * 4), dtype=dtype)
 
 
 class BlockMatrix:
@@ -78,7 +75,7 @@ class BlockMatrix:
     the other order are laid out once, here. Padded ones must hold zeros from ``cols`` on.
     """
 
-    __slots__ = ("data", "scales", "rows", "cols", "block_rows")
+    __slots__ = ("data", "_room", "rows", "cols", "block_rows")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, cols: Optional[int] = None,
                  block_rows: int = 1) -> None:
@@ -109,22 +106,35 @@ class BlockMatrix:
         stride = (1, -(-rows // 8) * 8) if block_rows == 1 else (-(-kb // 4) * 4, 1)
         # (a view that has the strides by chance may end before its padding)
         if scales.stride() != stride or scales.data_ptr() % 16 or (rows % 8 if block_rows == 1 else kb % 4):
-            scales = _scales(*want, block_rows, scales.dtype, scales.device).copy_(scales)
-        self.data, self.scales, self.rows, self.cols, self.block_rows = values, scales, rows, cols, block_rows
+            room = _scales(scales, *want, block_rows, scales.dtype)
+            room[:want[0], :kb].copy_(scales)
+            scales = room
+        self.data, self._room, self.rows, self.cols, self.block_rows = values, scales, rows, cols, block_rows
 
     @classmethod
-    def _new(cls, rows: int, cols: int, block_rows: int, scale_dtype: torch.dtype, device) -> "BlockMatrix":
+    def _new(cls, x: torch.Tensor, block_rows: int, scale_dtype: torch.dtype) -> "BlockMatrix":
+        """Room for a block matrix of x's shape on its device."""
         m = cls.__new__(cls)
-        kb = blocks(cols)
-        m.data = torch.empty((rows, kb * BLOCK), dtype=E4M3, device=device)
-        m.scales = _scales(rows if block_rows == 1 else blocks(rows), kb, block_rows, scale_dtype, device)
+        rows, cols = x.shape
+        kb = (cols + 127) // 128
+        m.data = x.new_empty((rows, kb * BLOCK), dtype=E4M3)
+        m._room = _scales(x, rows if block_rows == 1 else (rows + 127) // 128, kb, block_rows, scale_dtype)
         m.rows, m.cols, m.block_rows = rows, cols, block_rows
         return m
 
     @property
     def values(self) -> torch.Tensor:
         """[rows, cols] e4m3: a view without the padding."""
-        return self.data[:, :self.cols]
+        return self.data if self.cols % BLOCK == 0 else self.data[:, :self.cols]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """[blocks of rows, blocks of columns]: a view without the padding."""
+        r, kb = self._room.shape
+        if self.block_rows == 1:
+            return self._room if r == self.rows else self._room[:self.rows]
+        want = self.data.shape[1] // BLOCK
+        return self._room if kb == want else self._room[:, :want]
 
     @property
     def shape(self) -> tuple[int, int]:
@@ -136,14 +146,13 @@ class BlockMatrix:
 
     def __repr__(self) -> str:
         return (f"BlockMatrix({self.rows}x{self.cols}, blocks {self.block_rows}x{BLOCK}, "
-                f"scales {self.scales.dtype}, {self.data.device})")
+                f"scales {self._room.dtype}, {self.data.device})")
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+_stream = torch._C._cuda_getCurrentRawStream     # current_stream(device) makes an object first: 1.8 us of a call of 10
 
 
-def _matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None) -> None:
+def _refuse_matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None) -> None:
     if t.dim() != 2 or t.stride(1) != 1 and t.shape[1] > 1:
         raise ValueError(f"{name}: a 2-D tensor whose columns are neighbours, not {tuple(t.shape)} "
                          f"with strides {t.stride()}")
@@ -154,8 +163,10 @@ def _matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None) -> 
 
 
 def _no_grad(*tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the 8-bit operators have no backward pass: call them under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the 8-bit operators have no backward pass: call them under torch.no_grad()")
 
 
 def _scale_kind(dtype: torch.dtype) -> int:
@@ -164,7 +175,7 @@ def _scale_kind(dtype: torch.dtype) -> int:
     return 1 if dtype is E8M0 else 0
 
 
-def _ok(rc: int, what: str) -> None:
+def _failed(rc: int, what: str) -> None:
     if rc < 0:
         raise ValueError(f"{what}: sizes out of range")
     hip._check(rc, what)
@@ -173,7 +184,7 @@ def _ok(rc: int, what: str) -> None:
 def quantize(x: torch.Tensor, block_rows: int = 1, scale_dtype: torch.dtype = torch.float32) -> BlockMatrix:
     """``x`` [rows, cols] (bfloat16, float16 or float32; any row stride) in e4m3 with a scale for
     each ``block_rows`` × 128 block: 1 for activations, 128 for weights."""
-    _matrix(x, "x")
+    _refuse_matrix(x, "x")
     _no_grad(x)
     pow2 = _scale_kind(scale_dtype)
     if block_rows not in (1, BLOCK):
@@ -181,9 +192,12 @@ def quantize(x: torch.Tensor, block_rows: int = 1, scale_dtype: torch.dtype = to
     rows, cols = x.shape
     if cols < 1:
         raise ValueError("x has no columns")
-    q = BlockMatrix._new(rows, cols, block_rows, scale_dtype, x.device)
-    _ok(_lib()[1](x.device.index, _stream(x.device), _TYPES[x.dtype], block_rows == BLOCK, pow2, x.data_ptr(),
-                  x.stride(0), q.data.data_ptr(), q.scales.data_ptr(), rows, cols), "fp8 quantize")
+    q = BlockMatrix._new(x, block_rows, scale_dtype)
+    device = x.get_device()
+    rc = _lib()[1](device, _stream(device), _TYPES[x.dtype], block_rows == BLOCK, pow2, x.data_ptr(), x.stride(0),
+                   q.data.data_ptr(), q._room.data_ptr(), rows, cols)
+    if rc:
+        _failed(rc, "fp8 quantize")
     return q
 
 
@@ -194,7 +208,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     Returns (y in e4m3 with 1 × 128 blocks, h); h is None without a residual. ``weight`` [cols] has
     x's type or is float32; x and residual [rows, cols] may have any row stride.
     """
-    _matrix(x, "x")
+    _refuse_matrix(x, "x")
     rows, cols = x.shape
     if cols < 1:
         raise ValueError("x has no columns")
@@ -205,18 +219,22 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     if weight.device != x.device:
         raise ValueError(f"x on {x.device}, weight on {weight.device}")
     if residual is not None:
-        _matrix(residual, "residual", x.dtype)
+        _refuse_matrix(residual, "residual", x.dtype)
         if residual.shape != x.shape or residual.device != x.device:
             raise ValueError(f"residual: {tuple(x.shape)} on {x.device}, not {tuple(residual.shape)} on {residual.device}")
     _no_grad(x, weight, residual)
     pow2 = _scale_kind(scale_dtype)
-    q = BlockMatrix._new(rows, cols, 1, scale_dtype, x.device)
-    h = None if residual is None else torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-    _ok(_lib()[0](x.device.index, _stream(x.device), _TYPES[x.dtype], weight.dtype == torch.float32, pow2,
-                  x.data_ptr(), x.stride(0), None if residual is None else residual.data_ptr(),
-                  0 if residual is None else residual.stride(0), weight.data_ptr(),
-                  None if h is None else h.data_ptr(), q.data.data_ptr(), q.scales.data_ptr(), rows, cols, eps),
-        "fp8 norm")
+    q = BlockMatrix._new(x, 1, scale_dtype)
+    device = x.get_device()
+    if residual is None:
+        h, res, r_pitch, to = None, None, 0, None
+    else:
+        h = torch.empty_like(x) if x.is_contiguous() else x.new_empty((rows, cols))
+        res, r_pitch, to = residual.data_ptr(), residual.stride(0), h.data_ptr()
+    rc = _lib()[0](device, _stream(device), _TYPES[x.dtype], weight.dtype == torch.float32, pow2, x.data_ptr(),
+                   x.stride(0), res, r_pitch, weight.data_ptr(), to, q.data.data_ptr(), q._room.data_ptr(), rows, cols, eps)
+    if rc:
+        _failed(rc, "fp8 norm")
     return q, h
 
 
@@ -233,8 +251,9 @@ def matmul(a: BlockMatrix, b: BlockMatrix, out_dtype: torch.dtype = torch.bfloat
         raise ValueError(f"a has blocks of {a.block_rows} row(s) and b of {b.block_rows}: 1 and {BLOCK} are wanted")
     if a.cols != b.cols:
         raise ValueError(f"a has {a.cols} columns, b {b.cols}")
-    if a.scales.dtype != b.scales.dtype:
-        raise TypeError(f"a's scales are {a.scales.dtype}, b's {b.scales.dtype}")
+    kind = a._room.dtype
+    if kind != b._room.dtype:
+        raise TypeError(f"a's scales are {kind}, b's {b._room.dtype}")
     device = a.data.device
     if b.data.device != device:
         raise ValueError(f"a on {device}, b on {b.data.device}")
@@ -252,16 +271,18 @@ def matmul(a: BlockMatrix, b: BlockMatrix, out_dtype: torch.dtype = torch.bfloat
     if out is None:
         out = torch.empty((m, n), dtype=out_dtype, device=device)
     else:
-        _matrix(out, "out", out_dtype)
+        _refuse_matrix(out, "out", out_dtype)
         if out.shape != (m, n) or out.device != device or m > 1 and out.stride(0) < n:
             raise ValueError(f"out: {(m, n)} on {device} with rows apart, not {tuple(out.shape)} on {out.device} "
                              f"with strides {out.stride()}")
         _no_grad(out)
-    kb, pow2 = blocks(a.cols), a.scales.dtype is E8M0
+    kb, pow2 = (a.cols + 127) // 128, kind is E8M0
     room = _workspace(m, n, kb, pow2)
     ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
-    _ok(_lib()[2](device.index, _stream(device), _OUT[out_dtype], pow2, a.data.data_ptr(), a.scales.data_ptr(),
-                  b.data.data_ptr(), b.scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(),
-                  m, n, kb, max(out.stride(0), n), -(-m // 8) * 8, None if ws is None else ws.data_ptr(), room),
-        "fp8 matmul")
+    index = device.index
+    rc = _lib()[2](index, _stream(index), _OUT[out_dtype], pow2, a.data.data_ptr(), a._room.data_ptr(),
+                   b.data.data_ptr(), b._room.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(),
+                   m, n, kb, max(out.stride(0), n), (m + 7) // 8 * 8, ws.data_ptr() if room else None, room)
+    if rc:
+        _failed(rc, "fp8 matmul")
     return out
