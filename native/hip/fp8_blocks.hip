@@ -35,7 +35,7 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(v, __shfl_xor(v, 32));
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off);
   return v;
@@ -78,6 +78,19 @@ __device__ __forceinline__ uint2 to_e4m3(const float (&v)[kWidth], float inv) {
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, hi, false);
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, hi, true);
   return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+
+// v, to nearest, where the exact value is v + rest: the neighbour with an odd last bit instead if rest is not 0.
+// A later rounding to fewer bits is then that of the exact value.
+__device__ __forceinline__ float to_odd(float v, float rest) {
+  const int b = __float_as_int(v), step = (b ^ __float_as_int(rest)) >> 31 | 1;      // -1 toward 0, 1 away from it
+  return __int_as_float(rest != 0.f && !(b & 1) ? b + step : b);
+}
+
+// The first `keep` of eight bytes, zeros behind them.
+__device__ __forceinline__ uint2 clear_past(uint2 v, int keep) {
+  const uint64_t all = (uint64_t)v.y << 32 | v.x, kept = keep <= 0 ? 0 : all & (~0ull >> (64 - 8 * keep));
+  return make_uint2((uint32_t)kept, (uint32_t)(kept >> 32));
 }
 
 // Eight neighbours of a row from column c on; zeros from column `cols` on. The rows of a caller's
@@ -146,7 +159,7 @@ struct NormArgs {
 template <typename T, typename W, bool POW2, bool RES, int THREADS, int CHUNKS>
 __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
   constexpr int kWaves = THREADS / 64;
-  __shared__ float part[kWaves];
+  __shared__ double part[kWaves];
   const int64_t r = row_of(blockIdx.x, a.rows);
   if (r < 0) return;
   const T* x = (const T*)a.x + r * a.x_pitch;
@@ -182,15 +195,17 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
       for (int i = 0; i < kWidth; ++i) h[i] = 0.f;
     }
   }
-  sum = wave_sum(sum);
+  // a lane's squares are summed in float32, the lanes' sums and the root are taken in 64 bits
+  double total = wave_sum((double)sum);
   if constexpr (kWaves > 1) {
-    if ((tid & 63) == 0) part[tid >> 6] = sum;
+    if ((tid & 63) == 0) part[tid >> 6] = total;
     __syncthreads();
-    sum = 0.f;
+    total = 0.;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) sum += part[i];
+    for (int i = 0; i < kWaves; ++i) total += part[i];
   }
-  const float rstd = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(sum, (float)a.cols) + a.eps));
+  const double root = 1. / sqrt(total / a.cols + a.eps);
+  const float rstd = (float)root, rstd_low = (float)(root - rstd);
 
   uint8_t* q = (uint8_t*)a.values + r * (int64_t)a.padded;
 #pragma unroll
@@ -201,16 +216,45 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
     if (c < a.padded) {          // the 16 lanes of a block agree: padded is a multiple of 128
       if constexpr (CHUNKS == 0) take(c, h);
       if constexpr (RES) store8<T>(out, c, a.cols, h);
-      float y[kWidth], g[kWidth], amax = 0.f;
-      load8<W>(w, c, a.cols, g);
+      // Within a block the root cancels: with g = h * w, exact for 16-bit h and w,
+      //   y / s = 448 g / max |g|,  or for a power of two  y / s = g * (rstd / s),
+      // each with its first rounding's error added back and rounded to odd: the conversion that follows then
+      // gives the 8-bit value next to the quotient itself, also where float32 would round onto a border.
+      float g[kWidth], w8[kWidth], v[kWidth], gmax = 0.f;
+      load8<W>(w, c, a.cols, w8);
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) {
-        y[i] = h[i] * rstd * g[i];
-        if (c + i >= a.cols) y[i] = 0.f;      // 0 * NaN in a padded column
-        amax = fmaxf(amax, finite_abs(y[i]));
+        g[i] = h[i] * w8[i];
+        gmax = fmaxf(gmax, finite_abs(g[i]));
       }
-      const float s = scale_of<POW2>(row_max(amax));
-      *(uint2*)(q + c) = to_e4m3(y, __fdiv_rn(1.f, s));
+      gmax = row_max(gmax);
+      float amax = rstd == rstd ? fminf(gmax * rstd, 3.402823466e38f) : 0.f;   // a NaN in the row: NaN values, scale 1
+      // a product that was rounded down onto 448 * 2^p lies above it
+      if (POW2 && fmaf(gmax, rstd, -amax) + gmax * rstd_low > 0.f && amax < 3.4e38f)
+        amax = __uint_as_float(__float_as_uint(amax) + 1);
+      const float s = scale_of<POW2>(amax);
+      const float f = rstd * __fdiv_rn(1.f, s), low = rstd_low * __fdiv_rn(1.f, s);
+      // (a scale at its least, and magnitudes that 448 or the inverse would take out of range, go the second way)
+      if (!POW2 && amax > 0.f && s > 1.17549435e-38f && gmax > 1e-30f && gmax < 1e30f) {
+        const float inv = __fdiv_rn(1.f, gmax);
+#pragma unroll
+        for (int i = 0; i < kWidth; ++i) {
+          const float top = g[i] * 448.f, first = top * inv;
+          const float rest = fmaf(-first, gmax, top);
+          v[i] = fabsf(rest) < 1e30f ? fmaf(rest, inv, first) : first;   // NaN and infinity as they are
+          v[i] = to_odd(v[i], fmaf(-v[i], gmax, top));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kWidth; ++i) {
+          const float rest = g[i] * low;
+          v[i] = fabsf(rest) < 1e30f ? fmaf(g[i], f, rest) : g[i] * f;
+          v[i] = to_odd(v[i], fmaf(g[i], f, -v[i]) + rest);
+        }
+      }
+      uint2 out8 = to_e4m3(v, 1.f);
+      if (c + kWidth > a.cols) out8 = clear_past(out8, a.cols - c);      // 0 * NaN in a padded column
+      *(uint2*)(q + c) = out8;
       if (tid % kLanes == 0) put_scale<POW2>(a.scales, (int64_t)(c / kBlockK) * a.s_pitch + r, s);
     }
   }
