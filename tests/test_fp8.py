@@ -84,3 +84,63 @@ def test_scale_dtype_and_gradients_are_refused():
 def test_matmul_refuses(a, b, kw, error):
     with pytest.raises(error):
         fp8.matmul(a, b, **kw)
+
+
+class FakeProber:
+    """A node's probes without a GPU: HIP ordinal d is amd-smi index d."""
+
+    def __init__(self, backend, wrong=(), nbytes=1 << 28):
+        self.backend, self.wrong, self.nbytes, self.runs = backend, set(wrong), nbytes, []
+
+    def count(self):
+        return self.backend.count
+
+    def bus_id(self, d):
+        return self.backend._bdf(d)
+
+    def bandwidth_gbps(self, d, nbytes):
+        return 6000.0
+
+    def pattern_errors(self, d, nbytes):
+        return 0
+
+    def matrix_bytes(self):
+        return self.nbytes
+
+    def matrix(self, d):
+        self.runs.append(d)
+        return (5 if d in self.wrong else 0), 2500.0
+
+
+def test_matrix_probe_counts_towards_health():
+    from yoda_scheduler_amd.sniffer.collector import FakeBackend
+    from yoda_scheduler_amd.sniffer.publisher import SnifferAgent
+    be = FakeBackend(4, node="n")
+    be.tenants[1] = (1, 32)                       # a tenant: not probed
+    prober = FakeProber(be, wrong={2})
+    agent = SnifferAgent(None, "n", be, probe=True, prober=prober, fail_threshold=2, probe_matrix=True)
+    for k in range(2):
+        res = agent.run_probes()
+    health = {c.id: c.health for c in agent.build().status.card_list}
+    assert health == {0: "Healthy", 1: "Healthy", 2: "Unhealthy", 3: "Healthy"}
+    assert prober.runs == [0, 2, 3] * 2 and res[2]["matrix_errors"] == 5 and res[2]["pattern_errors"] == 0
+    assert agent.measured_tflops == {0: 2500.0, 2: 2500.0, 3: 2500.0}
+    prober.wrong.clear()
+    agent.run_probes()
+    assert {c.health for c in agent.build().status.card_list} == {"Healthy"}
+
+
+def test_matrix_probe_is_off_by_default_and_keeps_to_its_share_of_memory():
+    from yoda_scheduler_amd.sniffer.collector import FakeBackend
+    from yoda_scheduler_amd.sniffer.publisher import SnifferAgent
+    be = FakeBackend(2, node="n")
+    prober = FakeProber(be)
+    res = SnifferAgent(None, "n", be, probe=True, prober=prober).run_probes()
+    assert not prober.runs and "matrix_errors" not in res[0]
+    prober = FakeProber(be, nbytes=(be.spec.hbm_mb // 4 + 1) << 20)
+    agent = SnifferAgent(None, "n", be, probe=True, prober=prober, probe_matrix=True)
+    res = agent.run_probes()
+    assert not prober.runs and res[0]["matrix_skipped"] and res[0]["fail_streak"] == 0
+    from yoda_scheduler_amd.cmd.sniffer import build_parser
+    assert build_parser().parse_args([]).probe_matrix is False
+    assert build_parser().parse_args(["--probe", "--probe-matrix"]).probe_matrix is True

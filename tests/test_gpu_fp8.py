@@ -426,3 +426,36 @@ def test_offsets_past_32_bits(require_gpu, m):
     _check_matmul(out[:, some.to(DEV)], a, small)
     out[:, some.to(DEV)] = 0
     assert not out.any()
+
+
+@pytest.mark.parametrize("pow2", [False, True])
+@pytest.mark.parametrize("rows,cols,inner", [(1, 256, 128), (37, 512, 384), (300, 768, 1024), (1, 8192, 2048)])
+def test_matrix_check_is_clean(require_gpu, rows, cols, inner, pow2):
+    from yoda_scheduler_amd.ops import hip
+    r = hip.matrix_check(0, rows, cols, inner, iters=3, pow2=pow2)
+    assert r["errors"] == 0 and r["tflops"] > 0, r
+
+
+def test_matrix_check_compares(require_gpu):
+    """Checkers that go by another seed's inputs: nearly every value of the norm and the weight is off, and the
+    checkers of a verifier that compares say so."""
+    from yoda_scheduler_amd.ops import hip
+    rows, cols, inner = 64, 512, 512
+    bad = hip.matrix_check(0, rows, cols, inner, iters=1, seed=1, verify_seed=77)
+    assert bad["errors"] > 0.8 * (rows + cols) * inner, bad
+    with pytest.raises(ValueError):
+        hip.matrix_check(0, 16, 300, 512)
+
+
+def test_matrix_check_rate(require_gpu):
+    from yoda_scheduler_amd.ops import hip
+    r = hip.matrix_check(0, iters=10)
+    # 4096 x 4096 x 4096 reaches 2500 TFLOP/s (float32 vector code would stay under 160)
+    assert r["errors"] == 0 and r["tflops"] > 1000, r
+    assert hip.matrix_check_bytes() > 4096 * 4096 * 14
+
+
+def test_prober_runs_the_matrix_check(require_gpu):
+    from yoda_scheduler_amd.sniffer.publisher import HipProber
+    wrong, rate = HipProber().matrix(0)
+    assert wrong == 0 and rate > 1000

@@ -5,7 +5,8 @@ Samples every GPU of the node with the C++ amd-smi collector every ``--interval`
 and publishes the node's ``Scv`` status when something the scheduler acts on changed
 (or every ``--heartbeat`` seconds). With ``--probe`` the gfx950 HBM probes run on idle
 GPUs every ``--probe-interval`` seconds (measured bandwidth → ``Card.Bandwidth``,
-``--probe-fail-threshold`` consecutive pattern failures → ``Card.Health`` Unhealthy).
+``--probe-fail-threshold`` consecutive pattern failures → ``Card.Health`` Unhealthy);
+``--probe-matrix`` adds a checked 8-bit linear layer on the matrix cores to them.
 ``--print`` samples once and prints the Scv JSON (no apiserver needed).
 """
 from __future__ import annotations
@@ -35,6 +36,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--backend", choices=["amd-smi", "fake"], default="amd-smi")
     p.add_argument("--fake-gpus", type=int, default=8)
     p.add_argument("--probe", action="store_true", help="run the HIP HBM bandwidth/pattern probes on idle GPUs")
+    p.add_argument("--probe-matrix", action="store_true",
+                   help="with --probe: also run an 8-bit linear layer on idle GPUs and check every value of it")
     p.add_argument("--probe-bytes", type=int, default=1 << 30, help="upper bound (also ≤ 25%% of free HBM)")
     p.add_argument("--probe-interval", type=float, default=600.0, help="re-probe idle GPUs every N seconds")
     p.add_argument("--probe-fail-threshold", type=int, default=3,
@@ -57,7 +60,8 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     backend = make_backend(a.backend, a.fake_gpus)
     if a.print_only:
         agent = SnifferAgent(None, a.node, backend, a.interval, probe=a.probe, probe_bytes=a.probe_bytes,
-                             heartbeat=a.heartbeat, fail_threshold=a.probe_fail_threshold)
+                             heartbeat=a.heartbeat, fail_threshold=a.probe_fail_threshold,
+                             probe_matrix=a.probe_matrix)
         if a.probe:
             agent.run_probes()
         print(json.dumps(agent.build().to_json(), indent=2))
@@ -68,7 +72,8 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
         client = KubeClient(KubeConfig.load(a.kubeconfig, a.master))
         agent = SnifferAgent(client, a.node, backend, a.interval, probe=a.probe, probe_bytes=a.probe_bytes,
                              heartbeat=a.heartbeat, free_delta_mb=a.free_delta_mb, load_delta=a.load_delta,
-                             probe_interval=a.probe_interval, fail_threshold=a.probe_fail_threshold)
+                             probe_interval=a.probe_interval, fail_threshold=a.probe_fail_threshold,
+                             probe_matrix=a.probe_matrix)
         try:
             await agent.run(count=a.count or None)
         finally:

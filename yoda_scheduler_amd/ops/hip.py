@@ -51,6 +51,8 @@ def _declare(lib: ctypes.CDLL) -> None:
         "yoda_fp8_matmul": [c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                             c_int64, c_int64, c_int, c_int64, c_int64, c_void_p, c_int64],
         "yoda_fp8_matmul_workspace": [c_int64, c_int64, c_int, c_int],
+        "yoda_fp8_matrix_check": [c_int, c_int64, c_int64, c_int, c_int, c_int, c_uint, c_uint, P(c_double), P(c_ull)],
+        "yoda_fp8_matrix_check_bytes": [c_int64, c_int64, c_int],
     }
     for name, args in sigs.items():
         f = getattr(lib, name, None)
@@ -59,7 +61,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         if f is None:
             raise AttributeError(f"{PATH} has no {name}")
         f.argtypes = args
-        f.restype = c_int64 if name.endswith("_workspace") else c_int
+        f.restype = c_int64 if name.endswith(("_workspace", "_bytes")) else c_int
     try:
         from . import device_scorer as _ds
     except ImportError:
@@ -145,6 +147,29 @@ def peer_write_bandwidth(src: int, dst: int, nbytes: int = 256 << 20, iters: int
     _check(lib().yoda_peer_write_bandwidth(src, dst, nbytes, iters, ctypes.byref(g), ctypes.byref(sup)),
            "peer_write_bandwidth")
     return {"gbps": g.value, "supported": bool(sup.value)}
+
+
+def matrix_check(device: int = 0, rows: int = 4096, cols: int = 4096, inner: int = 4096, iters: int = 10,
+                 pow2: bool = True, seed: int = 0x5eed, verify_seed: int | None = None) -> dict:
+    """Run an 8-bit linear layer of the sizes given (:mod:`.fp8`: residual + norm, a weight's blocks, their
+    product), check every value against plain vector code and time the product. ``errors`` counts
+    values that are wrong or that change from one repetition to the next; ``verify_seed`` ≠ ``seed`` is the
+    checkers' self-test (the norm's and the weight's values must mismatch)."""
+    rate, err = c_double(0), c_ull(0)
+    vs = seed if verify_seed is None else verify_seed
+    rc = lib().yoda_fp8_matrix_check(device, rows, cols, inner, iters, int(pow2), seed, vs, ctypes.byref(rate),
+                                     ctypes.byref(err))
+    if rc < 0:
+        raise ValueError(f"matrix_check: {rows} rows (1 to 65535), {cols} columns (a multiple of 256) and {inner} "
+                         "inner (a multiple of 128) are out of range")
+    _check(rc, "matrix_check")
+    return {"errors": err.value, "tflops": rate.value, "rows": rows, "cols": cols, "inner": inner, "iters": iters,
+            "values": rows * inner + cols * inner + rows * cols}
+
+
+def matrix_check_bytes(rows: int = 4096, cols: int = 4096, inner: int = 4096) -> int:
+    """Device memory that :func:`matrix_check` of these sizes takes."""
+    return int(lib().yoda_fp8_matrix_check_bytes(rows, cols, inner))
 
 
 def occupy(device: int = 0, ms: int = 1000) -> int:

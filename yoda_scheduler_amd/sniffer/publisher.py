@@ -14,7 +14,9 @@ a 409), so an idle 1000-node cluster costs ~1000/heartbeat writes/s instead of 2
 HBM probes (gfx950 kernels, ``native/hip/probes.hip``) run only on idle GPUs (no tenant
 process and little HBM in use), with a buffer sized from the free HBM, and are repeated
 every ``probe_interval``; a GPU turns Unhealthy after ``fail_threshold`` consecutive
-failed pattern checks and recovers after a clean one. Probe results are attributed to
+failed pattern checks and recovers after a clean one. With ``probe_matrix`` an 8-bit linear
+layer (``native/hip/fp8_probe.hip``) runs after them, checked value by value, and counts
+like a failed pattern check where a value is wrong. Probe results are attributed to
 amd-smi indices through the HIP ordinal ↔ amd-smi mapping (``hipId`` from
 ``amdsmi_get_gpu_enumeration_info``, else the PCI bus id), never by assuming the two
 enumerations agree.
@@ -78,13 +80,23 @@ class HipProber:
         from ..ops import hip
         return int(hip.hbm_pattern_check(d, nbytes)["errors"])
 
+    def matrix_bytes(self) -> int:
+        from ..ops import hip
+        return hip.matrix_check_bytes()
+
+    def matrix(self, d: int) -> tuple[int, float]:
+        """(wrong or unstable values, TFLOP/s) of an 8-bit linear layer on the card."""
+        from ..ops import hip
+        r = hip.matrix_check(d)
+        return int(r["errors"]), float(r["tflops"])
+
 
 class SnifferAgent:
     def __init__(self, client, node: str, backend, interval: float = 1.0, probe: bool = False,
                  probe_bytes: int = 1 << 30, heartbeat: float = 10.0, free_delta_mb: int = 1024,
                  load_delta: float = 0.05, occupancy_delta: float = 5.0, probe_interval: float = 600.0,
                  probe_max_fraction: float = 0.25, busy_vram_mb: int = 2048, fail_threshold: int = 3,
-                 prober=None, clock=time.monotonic) -> None:
+                 prober=None, clock=time.monotonic, probe_matrix: bool = False) -> None:
         self.client = client
         self.node = node
         self.backend = backend
@@ -100,9 +112,11 @@ class SnifferAgent:
         self.busy_vram_mb = busy_vram_mb
         self.fail_threshold = max(1, fail_threshold)
         self.prober = prober
+        self.probe_matrix = probe_matrix
         self.clock = clock
         # probe state per amd-smi index
         self.measured_bw: dict[int, float] = {}
+        self.measured_tflops: dict[int, float] = {}
         self.probe_fail_streak: dict[int, int] = {}
         self.probe_runs: dict[int, int] = {}
         self.probe_skipped: dict[int, str] = {}
@@ -150,11 +164,21 @@ class SnifferAgent:
             self.probe_skipped.pop(i, None)
             bw = prober.bandwidth_gbps(d, nbytes)
             errs = prober.pattern_errors(d, nbytes)
+            matrix: dict = {}
+            if self.probe_matrix:
+                # within the fraction of the free HBM that the memory probes keep to
+                if prober.matrix_bytes() > int(free_mb * self.probe_max_fraction) << 20:
+                    matrix = {"matrix_skipped": "too little free HBM"}
+                else:
+                    wrong, tflops = prober.matrix(d)
+                    self.measured_tflops[i] = tflops
+                    matrix = {"matrix_errors": wrong, "matrix_tflops": tflops}
             self.measured_bw[i] = round(bw)
-            self.probe_fail_streak[i] = self.probe_fail_streak.get(i, 0) + 1 if errs else 0
+            failed = errs or matrix.get("matrix_errors", 0)
+            self.probe_fail_streak[i] = self.probe_fail_streak.get(i, 0) + 1 if failed else 0
             self.probe_runs[i] = self.probe_runs.get(i, 0) + 1
             res[i] = {"hip": d, "bytes": nbytes, "read_gbps": bw, "pattern_errors": errs,
-                      "fail_streak": self.probe_fail_streak[i]}
+                      "fail_streak": self.probe_fail_streak[i], **matrix}
         return res
 
     async def maybe_probe(self, samples: list[dict]) -> Optional[dict]:
