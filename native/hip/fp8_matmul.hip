@@ -799,13 +799,14 @@ int narrow(const MatArgs& p, bool pow2, hipStream_t s) {
 
 // ---------------------------------------------------------------- which one
 //
-// By sizes alone, the least of these estimates (us; what the kernels took on an MI355X, sums to 5 TB/s):
-//   few rows    2 + (weight + rows for every 32 columns) / 8 MB           (64 x 8192 x 8192: 24)
-//   128 x 128   5.5 + steps * (0.47, or 0.95 a round of 512 workgroups, float scales 1.1)
-//               + 3 + twice the parts' bytes / 5 MB where K has parts     (777 x 5000 x 1928: 17, 27 with 256 x 256;
-//                                                                          128 x 8192 x 4096 in 2 parts 17, in 1 21)
-//   256 x 256   rounds of 256 * (8 + steps * (1.45, float scales 1.6)),   (4096 x 4096 x 4096: 55, 65 with 128 x 128;
-//               a last round of a share f of them counts (1 + f) / 2       4096 x 10240 x 4096: 163, 194 with 128 x 128)
+// By sizes alone, the least of these estimates in us, fitted to what the kernels take on an MI355X:
+//   few rows    2 + (weight + rows for every 32 columns) / 8 MB
+//   128 x 128   up to 256 workgroups 5.5 + 0.55 a step, else 2 + (4.5 + 0.9 a step) a round of 512;
+//               K in parts: 3 more for the join, and twice the parts' bytes / 5 MB
+//   256 x 256   (10.5 + 1.4 a step) a round of 256; a last round of a share f of them counts (1 + f) / 2
+// (float scales: 0.95 and 1.57 a step). Measured both ways, 128 x 128 against 256 x 256, e8m0 scales:
+//   2048 x 2048 x 4096 23 : 44, 777 x 5000 x 1928 17 : 27, 4096 x 4096 x 512 18.0 : 17.4, 4096 x 4096 x 4096 64 : 55,
+//   8192 x 8192 x 4096 293 : 223;  few rows against 128 x 128: 32 x 8192 x 8192 17 : 21, 128 x 8192 x 4096 21 : 17.
 struct Plan {
   enum { kNarrow, kMid, k256 } kind;
   int parts;
@@ -817,7 +818,7 @@ Plan plan(int64_t m, int64_t n, int kb, bool pow2) {
   Plan best = {Plan::k256, 1, 0};
   const int64_t big = (m + 255) / 256 * ((n + 255) / 256), tiles = (m + 127) / 128 * ((n + 127) / 128);
   const double rest = big % 256 ? (1 + big % 256 / 256.0) / 2 : 0;
-  double least = (std::max<double>(big / 256 + rest, 1)) * (8 + kb * (pow2 ? 1.45 : 1.6));
+  double least = std::max<double>(big / 256 + rest, 1) * (10.5 + kb * (pow2 ? 1.4 : 1.57));
   if (m <= 64) {
     const int rows = m <= 16 ? 16 : m <= 32 ? 32 : 64;
     const double t = 2 + weight * (1 + rows / 32.0) / 8e6;
@@ -827,8 +828,9 @@ Plan plan(int64_t m, int64_t n, int kb, bool pow2) {
     if (parts > 1 && tiles * parts > 512) break;
     const int64_t bytes = parts > 1 ? tiles * parts * 128 * 128 * 4 : 0;
     const int steps = (kb + parts - 1) / parts;
-    const double step = tiles * parts <= 256 ? 0.47 : (double)((tiles * parts + 511) / 512) * (pow2 ? 0.95 : 1.1);
-    const double t = 5.5 + steps * step + (parts > 1 ? 3 + 2 * bytes / 5e6 : 0);
+    const double rounds = (double)((tiles * parts + 511) / 512);
+    double t = tiles * parts <= 256 ? 5.5 + steps * 0.55 : 2 + rounds * (4.5 + steps * (pow2 ? 0.9 : 0.95));
+    if (parts > 1) t += 3 + 2 * bytes / 5e6;
     if (t < least) least = t, best = {Plan::kMid, parts, bytes};
   }
   return best;

@@ -248,6 +248,53 @@ def test_matmul_of_whole_numbers_is_exact(require_gpu, m, n, k, pow2):
 
 
 @pytest.mark.parametrize("pow2", [False, True])
+@pytest.mark.parametrize("k", [100, 250, 380, 1300, 1500])
+def test_matmul_large(require_gpu, k, pow2):
+    """Sizes that take the large tiles, at the edges of rows, columns and K; the reference in float64 on the GPU."""
+    fp8 = _ops()
+    m, n = 3900, 4001
+    sd = E8M0 if pow2 else torch.float32
+    a = fp8.quantize(_randn((m, k), k).to(DEV), 1, sd)
+    b = fp8.quantize((_randn((n, k), k + 1, spread=0) / k ** 0.5).to(DEV), 128, sd)
+    bias = _randn((n,), 7, torch.bfloat16)
+    da, db = (_dequantized(x).to(DEV) for x in (a, b))
+    want = torch.mm(da, db.t().contiguous()) + bias.to(DEV).double()
+    mass = torch.mm(da.abs(), db.abs().t().contiguous()) + bias.to(DEV).double().abs()
+    largest = torch.zeros(m, n, device=DEV)
+    xa, xb = (torch.nn.functional.pad(d.abs(), (0, -k % 8)).float() for d in (da, db))
+    for i in range(0, xa.shape[1], 8):
+        largest += (xa[:, None, i:i + 8] * xb[None, :, i:i + 8]).amax(2)
+    room = 7 * 2.0 ** -13 * largest.double() * (1 + 2.0 ** -12) + 2 * (k + 2) * 2.0 ** -24 * mass
+    room = room + (want.abs() + room) * 2.0 ** -8
+    out = fp8.matmul(a, b, torch.bfloat16, bias.to(DEV))
+    assert ((out.double() - want).abs() <= room).all()
+
+
+@pytest.mark.parametrize("m,n,k,pow2", [(3000, 4001, 8500, False), (2900, 3900, 33_000, True), (2900, 3900, 16_700, False),
+                                        (200, 2000, 9000, False), (40, 3000, 40_000, True), (3900, 4001, 3 * 128, True)])
+def test_matmul_of_whole_numbers_is_exact_over_long_sums(require_gpu, m, n, k, pow2):
+    """Scales are held for 64 or 256 steps at a time: sums longer than that, exact as above."""
+    fp8 = _ops()
+    g = torch.Generator(device=DEV).manual_seed(k)
+    kb = fp8.blocks(k)
+
+    def whole(low, high, *shape):
+        return torch.randint(low, high + 1, shape, generator=g, device=DEV)
+
+    qa, qb = whole(-1, 1, m, k).float(), whole(-1, 1, n, k).float()
+    sa, sb = 2.0 ** whole(-1, 1, m, kb).float(), 2.0 ** whole(-1, 1, fp8.blocks(n), kb).float()
+    sd = E8M0 if pow2 else torch.float32
+    a = fp8.BlockMatrix(qa.to(E4M3), sa.to(sd))
+    b = fp8.BlockMatrix(qb.to(E4M3), sb.to(sd), block_rows=128)
+    da = qa.double() * sa.double().repeat_interleave(128, 1)[:, :k]
+    db = qb.double() * sb.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+    want = torch.mm(da, db.t().contiguous())
+    assert want.abs().max() * 4 < 2 ** 24 and (want * 4 == (want * 4).round()).all()
+    got = fp8.matmul(a, b, torch.bfloat16)
+    assert torch.equal(got, want.float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("pow2", [False, True])
 @pytest.mark.parametrize("m,n", [(3, 70), (40, 200), (130, 520), (300, 300)])
 def test_matmul_writes_its_rows_alone(require_gpu, m, n, pow2):
     """A wider, longer buffer: what lies beside and behind the output stays."""
