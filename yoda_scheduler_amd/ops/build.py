@@ -7,7 +7,10 @@
 * ``_yoda_sniffer`` C++ amd-smi collector (pybind11, links libamd_smi)  native/sniffer/
 * ``yoda-sniffer``  standalone collector binary (JSON on stdout)        native/sniffer/
 * ``libyoda_hip``   gfx950 HIP kernels: batched placement scorer, HBM /
-                    xGMI probes (hipcc --offload-arch=gfx950, C ABI)    native/hip/
+                    xGMI / matrix probes, 8-bit operators
+                    (hipcc --offload-arch=gfx950, C ABI)                native/hip/
+* ``_yoda_fp8``     the 8-bit operators' calls on torch tensors (CPython
+                    extension; only where torch is installed)           native/fp8/
 
 Outputs land in ``yoda_scheduler_amd/_native/`` so they travel with the repo snapshot
 to the GPU box.
@@ -25,6 +28,7 @@ from __future__ import annotations
 
 import argparse
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -67,6 +71,8 @@ ARTEFACTS: dict[str, dict] = {
                     "deps": ["sniffer/collector.cpp", "sniffer/collector.hpp", "sniffer/main.cpp",
                              "common/build_id.h"],
                     "recipe": "g++ -O2 -std=c++17 -lamd_smi v2"},
+    "fp8": {"out": f"_yoda_fp8{EXT}", "srcs": ["fp8/bindings.cpp"], "deps": ["fp8/bindings.cpp", "common/build_id.h"],
+            "recipe": "g++ -O2 -std=c++17 -fPIC -shared -fvisibility=hidden -ltorch_python v1"},
     "hip": {"out": "libyoda_hip.so", "srcs": None, "deps": None,     # every native/hip/*.hip + *.h
             "recipe": f"hipcc --offload-arch={ARCH} -O3 -std=c++17 -fPIC -shared -packed-fp32-ops v3"},
 }
@@ -222,8 +228,32 @@ def build_hip(force: bool = False) -> Path:
     return out
 
 
+def torch_root() -> Path | None:
+    """Where torch is installed (found without importing it), or None."""
+    spec = importlib.util.find_spec("torch")
+    return Path(spec.origin).parent if spec is not None and spec.origin else None
+
+
+def build_fp8(force: bool = False) -> list[Path]:
+    """The 8-bit operators' torch module; nothing where torch or its headers are missing (the scheduler's image)."""
+    torch = torch_root()
+    if torch is None or not (torch / "include" / "ATen" / "ATen.h").exists():
+        return []
+    out = out_path("fp8")
+    if force or _stale("fp8"):
+        bid = source_hash("fp8")
+        inc = [f"-I{torch / 'include'}", f"-I{torch / 'include/torch/csrc/api/include'}",
+               f"-I{sysconfig.get_paths()['include']}", f"-I{NATIVE / 'common'}"]
+        _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+              "-Wno-unused-function", "-D_GLIBCXX_USE_CXX11_ABI=1", _bid_flag(bid), *inc, *_srcs("fp8"), "-o", str(out),
+              f"-L{torch / 'lib'}", f"-Wl,-rpath,{torch / 'lib'}", "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python"],
+             "8-bit operators' torch module")
+        _record("fp8", bid)
+    return [out]
+
+
 BUILDERS = {"core": lambda f: [build_core(f)], "kube": build_kube, "fakeapi": build_kube,
-            "sniffer": build_sniffer, "sniffer_bin": build_sniffer, "hip": lambda f: [build_hip(f)]}
+            "sniffer": build_sniffer, "sniffer_bin": build_sniffer, "hip": lambda f: [build_hip(f)], "fp8": build_fp8}
 
 
 def verify_loaded(name: str, loaded_id: str, native: Path | None = None) -> None:
@@ -255,7 +285,7 @@ def ensure_fresh(name: str) -> None:
 
 def build_ids() -> dict:
     """{artefact: (recorded build id, source hash)} for every artefact (smoke / diagnostics)."""
-    return {n: (recorded_id(n), source_hash(n)) for n in ARTEFACTS}
+    return {n: (recorded_id(n), source_hash(n)) for n in ARTEFACTS if n != "fp8" or torch_root() is not None}
 
 
 def build_all(force: bool = False, hip: bool = True, sniffer: bool = True) -> list[Path]:
@@ -266,6 +296,7 @@ def build_all(force: bool = False, hip: bool = True, sniffer: bool = True) -> li
         jobs.append(lambda: build_sniffer(force))
     if hip:
         jobs.append(lambda: [build_hip(force)])
+        jobs.append(lambda: build_fp8(force))
     outs: list[Path] = []
     with ThreadPoolExecutor(len(jobs)) as ex:
         for r in ex.map(lambda f: f(), jobs):
