@@ -490,95 +490,121 @@ __device__ __forceinline__ void store4(const MatArgs& p, f32x4 v, int64_t m, int
   }
 }
 
-// ---------------------------------------------------------------- 128 x 128, K in parts
+// ---------------------------------------------------------------- smaller tiles, K in parts
 //
-// For products with too few tiles of 256 x 256 to fill the card: four waves of 64 x 64, a ring of STAGES steps in LDS, and
-// K in gridDim.y parts whose float32 sums go to a workspace and are joined by k_join in the order of the parts. With two
-// stages (66 KB) two workgroups share a CU and run while the other waits; with four, one has three steps of loads in flight.
+// For products with too few tiles of 256 x 256 to fill the card: four waves of 16*RP x 16*CP, two by two, and a ring of
+// STAGES steps in LDS. 128 x 128 is for many rows; 128, 64 or 32 rows x 32 columns for one row of tiles: every workgroup
+// reads all rows again (out of L2, 33 TB/s) and a piece of the weight (out of HBM) that nobody else reads.
+// K is in gridDim.y parts, whose float32 sums go to a workspace and are joined by k_join in the order of the parts. Where two
+// workgroups' stages fit in LDS, they share a CU and one runs while the other waits.
+template <int RP_, int CP_>
 struct Mid {
-  static constexpr int BM = 128, BN = 128;
-  static constexpr int kTile = 128 * kBlockK;                     // rows' or columns' step: 16 KB
-  static constexpr int kStage = 2 * kTile + 4 * 256;              // and each wave's rows' scales
-  static constexpr int kLoads = 9;                                // of a wave and step
+  static constexpr int RP = RP_, CP = CP_, BM = 32 * RP, BN = 32 * CP;
+  static constexpr int kRows = BM * kBlockK, kColumns = BN * kBlockK;         // a step's bytes
+  static constexpr int kStage = kRows + kColumns + 4 * 256;                   // and each wave's rows' scales
+  static constexpr int kLoads = RP + CP + 1;                                  // of a wave and step
+  static constexpr int kProducts = RP * CP, kSlots = kProducts > kLoads ? kProducts : kLoads;
 };
 
-// (LDS is given at the launch: with its size in the kernel the compiler would reckon with one workgroup on a CU for four
-// stages, spread the sums over the accumulation registers and move them to and fro every step.)
-template <int STAGES, typename O, bool POW2>
+// column c of piece j of CP: as in column_of where pieces pair up
+template <int CP>
+__device__ __forceinline__ constexpr int mid_column(int j, int c) {
+  return CP == 1 ? c : column_of(j, c);
+}
+
+// (LDS is given at the launch: with its size in the kernel the compiler would reckon with one workgroup on a CU,
+// spread the sums over the accumulation registers and move them to and fro every step.)
+template <int RP, int CP, int STAGES, typename O, bool POW2>
 __global__ __launch_bounds__(256, 2) void k_mid(MatArgs p, int tiles_m, int tiles_n, float* parts) {
-  using Q = Mid;
+  using Q = Mid<RP, CP>;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
   int tm, tn;
   if (!tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn)) return;
   const int64_t m0 = (int64_t)tm * Q::BM, n0 = (int64_t)tn * Q::BN, kp = (int64_t)p.kb * kBlockK;
-  const int64_t m = m0 + wm * 64 + c * 4, n = n0 + wn * 64;
+  const int64_t m = m0 + wm * 16 * RP + c * RP, n = n0 + wn * 16 * CP;
   const int first = __builtin_amdgcn_readfirstlane((uint32_t)p.kb * blockIdx.y / gridDim.y);
   const int end = __builtin_amdgcn_readfirstlane((uint32_t)p.kb * (blockIdx.y + 1) / gridDim.y);
 
   const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   const u32x4 rx = buffer_of(p.a + m0 * kp), rw = buffer_of(p.b + n0 * kp);
-  uint32_t vx[4], vw[4];
+  uint32_t vx[RP], vw[CP];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = (wave + 4 * i) * 8 + lane / 8, key = row >> 1 & 7, half = (row >> 6) * 64, at = row >> 4 & 3;
-    vx[i] = (uint32_t)(min((int64_t)half + (row & 15) * 4 + at, p.m - 1 - m0) * kp + ((lane & 7) ^ key) * 16);
-    vw[i] = (uint32_t)(min((int64_t)half + column_of(at, row & 15), p.n - 1 - n0) * kp + ((lane & 7) ^ key) * 16);
+  for (int i = 0; i < RP; ++i) {
+    const int row = (wave + 4 * i) * 8 + lane / 8, half = row / (16 * RP), piece = row / 16 % RP;
+    const int64_t at = half * 16 * RP + (row & 15) * RP + piece;
+    vx[i] = (uint32_t)(min(at, p.m - 1 - m0) * kp + ((lane & 7) ^ (row >> 1 & 7)) * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < CP; ++i) {
+    const int row = (wave + 4 * i) * 8 + lane / 8, half = row / (16 * CP), piece = row / 16 % CP;
+    const int64_t at = half * 16 * CP + mid_column<CP>(piece, row & 15);
+    vw[i] = (uint32_t)(min(at, p.n - 1 - n0) * kp + ((lane & 7) ^ (row >> 1 & 7)) * 16);
   }
   constexpr int kScale = POW2 ? 1 : 4;
-  // the wave's rows' scales: 64 floats, or bytes from the tile's first row on
+  // rows' scales: bytes from the tile's first row on, or 64 floats from the wave's first row (of 128) or the tile's
+  const int from = RP == 4 && !POW2 ? wm * 64 : 0;
   const uint32_t vs = POW2 ? (uint32_t)min((int64_t)lane * 4, p.sa_pitch - 4 - m0)
-                           : (uint32_t)min((int64_t)wm * 64 + lane, p.sa_pitch - 1 - m0) * 4;
-  auto fetch = [&](int k, int stage) {
+                           : (uint32_t)min((int64_t)from + lane, p.sa_pitch - 1 - m0) * 4;
+  // load number i of a step's
+  auto load = [&](int i, int k, int stage) {
     const uint32_t to = base + stage * Q::kStage;
-    const u32x4 rs = buffer_of((const uint8_t*)p.sa + (m0 + k * p.sa_pitch) * kScale);
-    load_lds<4>(if_any(rs, k < end), vs, 0, to + 2 * Q::kTile + wave * 256);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) load_lds<16>(if_any(rx, k < end), vx[i], k * kBlockK, to + (wave + 4 * i) * 1024);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) load_lds<16>(if_any(rw, k < end), vw[i], k * kBlockK, to + Q::kTile + (wave + 4 * i) * 1024);
+    if (i < RP) {
+      load_lds<16>(if_any(rx, k < end), vx[i < RP ? i : 0], k * kBlockK, to + (wave + 4 * i) * 1024);
+    } else if (i < RP + CP) {
+      load_lds<16>(if_any(rw, k < end), vw[i - RP], k * kBlockK, to + Q::kRows + (wave + 4 * (i - RP)) * 1024);
+    } else {
+      const u32x4 rs = buffer_of((const uint8_t*)p.sa + (m0 + k * p.sa_pitch) * kScale);
+      load_lds<4>(if_any(rs, k < end), vs, 0, to + Q::kRows + Q::kColumns + wave * 256);
+    }
   };
 
   const int piece = (g ^ (c >> 1)) * 16;
-  const uint8_t* lx = lds + (wm * 64 + c) * kBlockK;
-  const uint8_t* lw = lds + Q::kTile + (wn * 64 + c) * kBlockK;
-  const uint8_t* ls = lds + 2 * Q::kTile + wave * 256 + (POW2 ? wm * 64 + c * 4 : c * 16);
+  const uint8_t* lx = lds + (wm * 16 * RP + c) * kBlockK;
+  const uint8_t* lw = lds + Q::kRows + (wn * 16 * CP + c) * kBlockK;
+  const uint8_t* ls = lds + Q::kRows + Q::kColumns + wave * 256 + (wm * 16 * RP - from + c * RP) * kScale;
 
   // the columns' scale of a step, by scalar loads (address space 4): four bytes, or a float
   typedef const uint32_t __attribute__((address_space(4))) * Scalars;
   const Scalars sb = (Scalars)((const uint8_t*)p.sb + min(n, p.n - 1) / kBlockK * p.sb_pitch * kScale);
   auto column_scale = [&](int k) { return POW2 ? sb[k >> 2] >> (8 * (k & 3)) : sb[k]; };
 
-  f32x4 acc[4][4];
+  f32x4 acc[RP][CP];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < RP; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < CP; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
 #pragma unroll
-  for (int d = 0; d < STAGES; ++d) fetch(first + d, d);
+  for (int d = 0; d < STAGES; ++d)
+#pragma unroll
+    for (int i = 0; i < Q::kLoads; ++i) load(i, first + d, d);
   // operands of two steps: one in use, one being read
   struct Step {
-    i32x4 x[4][2], w[4][2];
-    f32x4 s;
+    i32x4 x[RP][2], w[CP][2];
+    float s[RP];
     uint32_t b, c;
   } step[2];
-  // read number `at` of 17: a step's first products need its first columns and all its rows
-  auto read = [&](Step& to, int from, int at) {
-    const int i = at / 2 % 4, h = at & 1, row = i * 16 * kBlockK + (h ? piece ^ 64 : piece);
-    if (at == 16) {
-      if constexpr (POW2) to.b = *(const uint32_t*)(ls + from);
-      else to.s = *(const f32x4*)(ls + from);
-    } else if (at < 8) {
-      to.x[i][h] = *(const i32x4*)(lx + from + row);
+  // read number `at`: the rows' pieces, the columns', the rows' scales
+  auto read = [&](Step& to, int stage, int at) {
+    const int h = (at & 1 ? piece ^ 64 : piece);
+    if (at < 2 * RP) {
+      to.x[at / 2][at & 1] = *(const i32x4*)(lx + stage + at / 2 * 16 * kBlockK + h);
+    } else if (at < 2 * (RP + CP)) {
+      to.w[at / 2 - RP][at & 1] = *(const i32x4*)(lw + stage + (at / 2 - RP) * 16 * kBlockK + h);
+    } else if constexpr (POW2) {
+      if constexpr (RP == 4) to.b = *(const uint32_t*)(ls + stage);
+      else if constexpr (RP == 2) to.b = *(const uint16_t*)(ls + stage);
+      else to.b = ls[stage];
     } else {
-      to.w[i][h] = *(const i32x4*)(lw + from + row);
+#pragma unroll
+      for (int i = 0; i < RP; ++i) to.s[i] = ((const float*)(ls + stage))[i];
     }
   };
   meet<(STAGES - 1) * Q::kLoads>();
 #pragma unroll
-  for (int at = 0; at < 17; ++at) read(step[0], 0, at);
+  for (int at = 0; at <= 2 * (RP + CP); ++at) read(step[0], 0, at);
   step[0].c = column_scale(first);
 
   int stage = 0;                                // step k's
@@ -586,34 +612,42 @@ __global__ __launch_bounds__(256, 2) void k_mid(MatArgs p, int tiles_m, int tile
     // step k is in this wave's registers, and after the meeting in every wave's; step k + 1 is in LDS
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     meet<(STAGES - 2) * Q::kLoads>();
-    const int ahead = stage + 1 < STAGES ? stage + 1 : 0, from = ahead * Q::kStage;
-    fetch(k + STAGES, stage);
+    const int ahead = stage + 1 < STAGES ? stage + 1 : 0, bytes = ahead * Q::kStage, free = stage;
     stage = ahead;
     next.c = column_scale(min(k + 1, end - 1));
-    f32x4 t[4], s;
-    if constexpr (!POW2) s = now.s * __uint_as_float(now.c);
-    auto add = [&](auto At) {
-      constexpr int at = decltype(At)::value, j = at / 4, i = at % 4;
+    f32x4 t[4];
+    float s[RP];
+    if constexpr (!POW2) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[i][r], s[i], acc[i][j][r]);
+      for (int i = 0; i < RP; ++i) s[i] = now.s[i] * __uint_as_float(now.c);
+    }
+    auto add = [&](auto At) {
+      constexpr int at = decltype(At)::value, j = at / RP, i = at % RP;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[at & 3][r], s[i], acc[i][j][r]);
     };
     auto one = [&](auto At) {
-      constexpr int at = decltype(At)::value, j = at / 4, i = at % 4;
-      if constexpr (POW2) {
-        acc[i][j] = mfma_scaled<i>(join(now.w[j]), join(now.x[i]), acc[i][j], now.c, now.b);
-      } else {
-        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        t[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(now.w[j]), join(now.x[i]), zero, 0, 0, 0, 0, 0, 0);
-        if constexpr (at >= 2) add(Index<at - 2>{});
+      constexpr int at = decltype(At)::value;
+      if constexpr (at < Q::kProducts) {
+        constexpr int j = at / RP, i = at % RP;
+        if constexpr (POW2) {
+          acc[i][j] = mfma_scaled<i>(join(now.w[j]), join(now.x[i]), acc[i][j], now.c, now.b);
+        } else {
+          const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+          t[at & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(now.w[j]), join(now.x[i]), zero, 0, 0, 0, 0, 0, 0);
+        }
       }
-      read(next, from, at);
-      if (at == 15) read(next, from, 16);
+      if constexpr (!POW2 && at >= 2 && at - 2 < Q::kProducts) add(Index<at - 2>{});
+      // the reads come early, so that they are done when the step ends
+      if (at < RP + CP) read(next, bytes, 2 * at), read(next, bytes, 2 * at + 1);
+      if (at == RP + CP) read(next, bytes, 2 * at);
+      if (at < Q::kLoads) load(at, k + STAGES, free);
       __builtin_amdgcn_sched_barrier(0);
     };
-    each<16>(one);
+    each<Q::kSlots>(one);
     if constexpr (!POW2) {
-      add(Index<14>{});
-      add(Index<15>{});
+      if constexpr (Q::kSlots - 2 < Q::kProducts) add(Index<Q::kSlots - 2>{});
+      if constexpr (Q::kSlots - 1 < Q::kProducts) add(Index<Q::kSlots - 1>{});
     }
   };
 #pragma unroll 1
@@ -623,53 +657,54 @@ __global__ __launch_bounds__(256, 2) void k_mid(MatArgs p, int tiles_m, int tile
   }
   if ((end - first) & 1) one_step(end - 1, step[0], step[1]);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing may reach LDS after the workgroup's end
-  if (!parts) {
-    store_tile<4, 4, O>(p, acc, m, n, g);
-    return;
+  if (parts) {
+    // this part's sums as they lie in the registers: each store a whole KB
+    f32x4* out = (f32x4*)parts + (((int64_t)blockIdx.y * tiles_m * tiles_n + (int64_t)tm * tiles_n + tn) * 4 + wave) * (RP * CP * 64) + lane;
+#pragma unroll
+    for (int i = 0; i < RP; ++i)
+#pragma unroll
+      for (int j = 0; j < CP; ++j) out[(i * CP + j) * 64] = acc[i][j];
+  } else if constexpr (CP == 1) {
+#pragma unroll
+    for (int i = 0; i < RP; ++i)
+      if (m + i < p.m && n + g * 4 < p.n) store4<O>(p, acc[i][0], m + i, n + g * 4);
+  } else {
+    store_tile<RP, CP, O>(p, acc, m, n, g);
   }
-  // this part's sums as they lie in the registers: each store a whole KB
-  f32x4* out = (f32x4*)parts + (((int64_t)blockIdx.y * tiles_m * tiles_n + (int64_t)tm * tiles_n + tn) * 4 + wave) * 1024 + lane;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) out[(i * 4 + j) * 64] = acc[i][j];
 }
 
-// out = the sum of the parts in their order, plus bias: four neighbours a lane, a tile every 16 workgroups.
-template <typename O>
+// out = the sum of the parts in their order, plus bias: four neighbours a lane, a tile every RP * CP workgroups.
+template <int RP, int CP, typename O>
 __global__ __launch_bounds__(256) void k_join(MatArgs p, int tiles_m, int tiles_n, const f32x4* parts, int count) {
-  const int tile = blockIdx.x / 16, at = blockIdx.x % 16 * 256 + threadIdx.x;
-  const int wave = at >> 10, i = at >> 8 & 3, j = at >> 6 & 3, c = at & 15, g = at >> 4 & 3;
-  const int64_t m = (int64_t)(tile / tiles_n) * 128 + (wave >> 1) * 64 + c * 4 + i;
-  const int64_t n = (int64_t)(tile % tiles_n) * 128 + (wave & 1) * 64 + (j >> 1) * 32 + g * 8 + (j & 1) * 4;
+  const int tile = blockIdx.x / (RP * CP), at = blockIdx.x % (RP * CP) * 256 + threadIdx.x;
+  const int wave = at / (RP * CP * 64), i = at / 64 / CP % RP, j = at / 64 % CP, c = at & 15, g = at >> 4 & 3;
+  const int64_t m = (int64_t)(tile / tiles_n) * (32 * RP) + (wave >> 1) * 16 * RP + c * RP + i;
+  const int64_t n = (int64_t)(tile % tiles_n) * (32 * CP) + (wave & 1) * 16 * CP +
+                    (CP == 1 ? g * 4 : (j >> 1) * 32 + g * 8 + (j & 1) * 4);
   if (m >= p.m || n >= p.n) return;
-  const f32x4* in = parts + (int64_t)tile * 4096 + at;
-  const int64_t apart = (int64_t)tiles_m * tiles_n * 4096;
+  const f32x4* in = parts + (int64_t)tile * (RP * CP * 256) + at;
+  const int64_t apart = (int64_t)tiles_m * tiles_n * (RP * CP * 256);
   f32x4 v = in[0];
   for (int k = 1; k < count; ++k) v += in[k * apart];
   store4<O>(p, v, m, n);
 }
 
-template <typename O>
+template <int RP, int CP, int STAGES, typename O>
 int run_mid(const MatArgs& p, bool pow2, int count, float* parts, hipStream_t s) {
-  const int64_t tm = (p.m + 127) / 128, tn = (p.n + 127) / 128, total = tm * tn;
+  using Q = Mid<RP, CP>;
+  const int64_t tm = (p.m + Q::BM - 1) / Q::BM, tn = (p.n + Q::BN - 1) / Q::BN, total = tm * tn;
   if (total > (1 << 26) || count > 65535) return -1;
   const dim3 grid((unsigned)((total + 7) / 8 * 8), count);
   float* to = count > 1 ? parts : nullptr;
-  if (total * count > 256) {
-    if (pow2) k_mid<2, O, true><<<grid, 256, 2 * Mid::kStage, s>>>(p, (int)tm, (int)tn, to);
-    else k_mid<2, O, false><<<grid, 256, 2 * Mid::kStage, s>>>(p, (int)tm, (int)tn, to);
-  } else {
-    if (pow2) k_mid<4, O, true><<<grid, 256, 4 * Mid::kStage, s>>>(p, (int)tm, (int)tn, to);
-    else k_mid<4, O, false><<<grid, 256, 4 * Mid::kStage, s>>>(p, (int)tm, (int)tn, to);
-  }
-  if (count > 1) k_join<O><<<(unsigned)(total * 16), 256, 0, s>>>(p, (int)tm, (int)tn, (const f32x4*)parts, count);
+  if (pow2) k_mid<RP, CP, STAGES, O, true><<<grid, 256, STAGES * Q::kStage, s>>>(p, (int)tm, (int)tn, to);
+  else k_mid<RP, CP, STAGES, O, false><<<grid, 256, STAGES * Q::kStage, s>>>(p, (int)tm, (int)tn, to);
+  if (count > 1) k_join<RP, CP, O><<<(unsigned)(total * RP * CP), 256, 0, s>>>(p, (int)tm, (int)tn, (const f32x4*)parts, count);
   return (int)hipGetLastError();
 }
 
 // ---------------------------------------------------------------- few rows
 //
-// Up to 64 rows the weight's bytes are what counts: one workgroup takes all rows and 16 * NP columns, its waves
+// Up to 16 rows the weight's bytes are what counts: one workgroup takes all rows and 16 * NP columns, its waves
 // take every WAVES-th block of K and read their operands from memory straight into registers, DEPTH
 // blocks ahead, each weight byte once on the whole card; the rows are read again by each workgroup, out of L2.
 // No wave waits for another until the end, when the waves' sums are added through LDS in the order of
@@ -799,39 +834,56 @@ int narrow(const MatArgs& p, bool pow2, hipStream_t s) {
 
 // ---------------------------------------------------------------- which one
 //
-// By sizes alone, the least of these estimates in us, fitted to what the kernels take on an MI355X:
-//   few rows    2 + (weight + rows for every 32 columns) / 8 MB
-//   128 x 128   up to 256 workgroups 5.5 + 0.55 a step, else 2 + (4.5 + 0.9 a step) a round of 512;
-//               K in parts: 3 more for the join, and twice the parts' bytes / 5 MB
-//   256 x 256   (10.5 + 1.4 a step) a round of 256; a last round of a share f of them counts (1 + f) / 2
-// (float scales: 0.95 and 1.57 a step). Measured both ways, 128 x 128 against 256 x 256, e8m0 scales:
-//   2048 x 2048 x 4096 23 : 44, 777 x 5000 x 1928 17 : 27, 4096 x 4096 x 512 18.0 : 17.4, 4096 x 4096 x 4096 64 : 55,
-//   8192 x 8192 x 4096 293 : 223;  few rows against 128 x 128: 32 x 8192 x 8192 17 : 21, 128 x 8192 x 4096 21 : 17.
+// By sizes alone, the least of the estimates below, in us, fitted to what the kernels take on an MI355X:
+//   up to 16 rows   2 + (weight + rows for every 32 columns) / 8 MB, and 3 for every further round of 256 workgroups
+//   small tiles     up to 256 workgroups 5 + `one` a step, else 2 + (`round` + `two` a step) a round of 512, and no
+//                   less than 3 + weight / 5.3 MB; K in parts: 2.5 more, and twice the parts' bytes / 5 MB
+//   256 x 256       (10.5 + 1.4 a step, float scales 1.57) a round of 256; a last round of a share f counts (1 + f) / 2
+// Measured, this one : the next best, e8m0 scales: 16 x 8192 x 8192 few rows 13.4 : 14.9 32 x 32;
+// 32 x 8192 x 8192 32 x 32 14.7 : 16.1 64 x 32; 64 x 8192 x 8192 64 x 32 15.3 : 16.7 64 x 64; 128 x 8192 x 4096 128 x 32
+// 11.9 : 15.2 128 x 128 in two parts; 2048 x 2048 x 4096 128 x 128 23 : 44 256 x 256; 4096 x 4096 x 4096 256 x 256
+// 55 : 64 128 x 128.
+struct Shape {
+  int rows, columns;                    // pieces of 32
+  double one, two, round;               // us a step alone on a CU, of two on a CU; and a round's own
+  double one_f, two_f;                  // with float scales
+};
+constexpr Shape kShapes[] = {
+    {4, 4, 0.44, 0.90, 4.5, 0.50, 0.95},
+    {4, 1, 0.215, 0.40, 2.5, 0.26, 0.45},
+    {2, 1, 0.16, 0.28, 2.5, 0.20, 0.33},
+    {1, 1, 0.15, 0.25, 2.5, 0.155, 0.25},
+};
+
 struct Plan {
-  enum { kNarrow, kMid, k256 } kind;
-  int parts;
-  int64_t bytes;                        // of workspace
+  enum { kNarrow, kSmall, k256 } kind;
+  int shape, parts;
+  int64_t groups, bytes;                // workgroups; bytes of workspace
 };
 
 Plan plan(int64_t m, int64_t n, int kb, bool pow2) {
   const double weight = (double)n * kb * kBlockK;
-  Plan best = {Plan::k256, 1, 0};
-  const int64_t big = (m + 255) / 256 * ((n + 255) / 256), tiles = (m + 127) / 128 * ((n + 127) / 128);
+  Plan best = {Plan::k256, 0, 1, 0, 0};
+  const int64_t big = (m + 255) / 256 * ((n + 255) / 256);
   const double rest = big % 256 ? (1 + big % 256 / 256.0) / 2 : 0;
   double least = std::max<double>(big / 256 + rest, 1) * (10.5 + kb * (pow2 ? 1.4 : 1.57));
-  if (m <= 64) {
-    const int rows = m <= 16 ? 16 : m <= 32 ? 32 : 64;
-    const double t = 2 + weight * (1 + rows / 32.0) / 8e6;
-    if (t < least) least = t, best = {Plan::kNarrow, 1, 0};
+  if (m <= 16) {
+    const double t = 2 + weight * 1.5 / 8e6 + 3. * ((n + 8191) / 8192 - 1);
+    if (t < least) least = t, best = {Plan::kNarrow, 0, 1, 0, 0};
   }
-  for (int parts = 1; parts <= 16 && parts * 2 <= kb; parts *= 2) {
-    if (parts > 1 && tiles * parts > 512) break;
-    const int64_t bytes = parts > 1 ? tiles * parts * 128 * 128 * 4 : 0;
-    const int steps = (kb + parts - 1) / parts;
-    const double rounds = (double)((tiles * parts + 511) / 512);
-    double t = tiles * parts <= 256 ? 5.5 + steps * 0.55 : 2 + rounds * (4.5 + steps * (pow2 ? 0.9 : 0.95));
-    if (parts > 1) t += 3 + 2 * bytes / 5e6;
-    if (t < least) least = t, best = {Plan::kMid, parts, bytes};
+  for (int shape = 0; shape < 4; ++shape) {
+    const Shape& h = kShapes[shape];
+    const int64_t tiles = (m + 32 * h.rows - 1) / (32 * h.rows) * ((n + 32 * h.columns - 1) / (32 * h.columns));
+    for (int parts = 1; parts <= 16 && parts * 2 <= std::max(kb, 2); parts *= 2) {
+      const int64_t groups = tiles * parts, bytes = parts > 1 ? groups * h.rows * h.columns * 4096 : 0;
+      if (parts > 1 && groups > 512) break;
+      const int steps = (kb + parts - 1) / parts;
+      const double rounds = (double)((groups + 511) / 512);
+      double t = groups <= 256 ? 5 + steps * (pow2 ? h.one : h.one_f) : 2 + rounds * (h.round + steps * (pow2 ? h.two : h.two_f));
+      t = std::max(t, 3 + weight / 5.3e6);
+      if (parts > 1) t += 2.5 + 2 * bytes / 5e6;
+      if (t < least) least = t, best = {Plan::kSmall, shape, parts, groups, bytes};
+    }
   }
   return best;
 }
@@ -841,11 +893,14 @@ int run(const MatArgs& p, bool pow2, float* workspace, int64_t bytes, hipStream_
   const Plan to = plan(p.m, p.n, p.kb, pow2);
   if (to.bytes > bytes || (to.bytes && !workspace)) return -1;
   if (to.kind == Plan::k256) return run_256<O>(p, pow2, s);
-  if (to.kind == Plan::kMid) return run_mid<O>(p, pow2, to.parts, workspace, s);
   // two pieces of columns a workgroup halve what is read of the rows, where that leaves enough workgroups
-  if (p.m <= 16) return p.n >= 8192 ? narrow<1, 2, 8, 4, O>(p, pow2, s) : narrow<1, 1, 8, 4, O>(p, pow2, s);
-  if (p.m <= 32) return narrow<2, 2, 8, 4, O>(p, pow2, s);
-  return narrow<4, 2, 8, 2, O>(p, pow2, s);
+  if (to.kind == Plan::kNarrow) return p.n >= 8192 ? narrow<1, 2, 8, 4, O>(p, pow2, s) : narrow<1, 1, 8, 4, O>(p, pow2, s);
+  // stages: those of one workgroup fill LDS where there is one on a CU, else those of two
+  const bool alone = to.groups <= 256;
+  if (to.shape == 0) return alone ? run_mid<4, 4, 4, O>(p, pow2, to.parts, workspace, s) : run_mid<4, 4, 2, O>(p, pow2, to.parts, workspace, s);
+  if (to.shape == 1) return alone ? run_mid<4, 1, 6, O>(p, pow2, to.parts, workspace, s) : run_mid<4, 1, 3, O>(p, pow2, to.parts, workspace, s);
+  if (to.shape == 2) return run_mid<2, 1, 5, O>(p, pow2, to.parts, workspace, s);
+  return run_mid<1, 1, 8, O>(p, pow2, to.parts, workspace, s);
 }
 
 }  // namespace

@@ -271,7 +271,13 @@ def test_matmul_large(require_gpu, k, pow2):
 
 
 @pytest.mark.parametrize("m,n,k,pow2", [(3000, 4001, 8500, False), (2900, 3900, 33_000, True), (2900, 3900, 16_700, False),
-                                        (200, 2000, 9000, False), (40, 3000, 40_000, True), (3900, 4001, 3 * 128, True)])
+                                        (200, 2000, 9000, False), (40, 3000, 40_000, True), (3900, 4001, 3 * 128, True),
+                                        # every shape of tile, whole and in parts of K
+                                        (3, 17_000, 700, True), (20, 100, 20_000, True), (20, 100, 20_000, False),
+                                        (31, 9000, 1500, False), (64, 512, 16_384, True), (64, 512, 16_384, False),
+                                        (50, 9000, 900, True), (100, 200, 12_000, True), (100, 200, 12_000, False),
+                                        (128, 9000, 640, False), (130, 130, 9000, True), (500, 900, 5000, False),
+                                        (512, 8192, 1000, True), (777, 5000, 500, False), (1024, 2000, 700, True)])
 def test_matmul_of_whole_numbers_is_exact_over_long_sums(require_gpu, m, n, k, pow2):
     """Scales are held for 64 or 256 steps at a time: sums longer than that, exact as above."""
     fp8 = _ops()
