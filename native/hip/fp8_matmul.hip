@@ -164,8 +164,9 @@ __device__ __forceinline__ void store_tile(const MatArgs& p, const f32x4 (&acc)[
 struct Quarters {
   static constexpr int BM = 256, BN = 256;
   static constexpr int kPart = 128 * kBlockK;                     // x0, x1, w0 or w1 of one step: 16 KB
-  static constexpr int kStep = 4 * kPart, kScales = 2 * kStep;    // then 4 steps x 4 waves x 256 scales
-  static constexpr int kLds = kScales + 4 * 4 * 256;
+  static constexpr int kStep = 4 * kPart, kScales = 2 * kStep;    // then 4 steps x 4 waves x 256 scales of rows
+  static constexpr int kHeld = kScales + 4 * 4 * 256;             // and each wave's columns' scales of 256 steps
+  static constexpr int kLds = kHeld + 4 * 256;
 };
 
 // wait for all but `left` of the wave's loads, then for the other waves
@@ -230,11 +231,13 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
     w[j][h] = *(const i32x4*)(lw + (k & 1) * Q::kStep + (j >> 2) * Q::kPart + (j & 3) * 16 * kBlockK + (h ? piece ^ 64 : piece));
   };
 
-  // the columns' scales of 256 steps: four in each lane
+  // the columns' scales of 256 steps: four in each lane, by way of LDS like all else, so that the compiler sees no
+  // load that it would wait for behind the others
   const uint8_t* sb = (const uint8_t*)p.sb + min(n0 + wn * 128, p.n - 1) / kBlockK * p.sb_pitch;
-  auto column_scales = [&](int k) { return ((const uint32_t*)sb)[min((k >> 2) + lane, last >> 2)]; };
-  uint32_t sbs = column_scales(0);
-  asm volatile("" : "+v"(sbs));
+  auto load_columns = [&](int k) {
+    load_lds<4>(buffer_of(sb + k), (uint32_t)min(lane, (last - k) >> 2) * 4, 0, base + Q::kHeld + wave * 256);
+  };
+  const uint32_t* held = (const uint32_t*)(lds + Q::kHeld + wave * 256) + lane;
 
   f32x4 acc[8][8];
 #pragma unroll
@@ -246,6 +249,7 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
 #pragma unroll
     for (int i = 0; i < 4; ++i) load(i);
   };
+  load_columns(0);
   load_s(0);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -256,6 +260,7 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
     four([&](int i) { load_x(1, i, k); });
   }
   meet<26>();
+  uint32_t sbs = *held;
   uint2 next = *(const uint2*)ls, now;
 #pragma unroll
   for (int i = 0; i < 4; ++i) read_x(0, i, 0), read_x(0, i, 1);
@@ -268,8 +273,9 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
 #pragma unroll 1
   for (int k = 0; k < p.kb; ++k) {
     if ((k & 255) == 0 && k) {
-      sbs = column_scales(k);
-      asm volatile("" : "+v"(sbs));
+      load_columns(k);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      sbs = *held;
     }
     // product number `at` of a quarter, one piece of columns after the other
     auto quarter = [&](auto Rows, auto Cols, auto between) {
@@ -327,8 +333,9 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
 struct Eight {
   static constexpr int BM = 256, BN = 256;
   static constexpr int kRows = 128 * kBlockK;                     // half of the rows' pieces: 16 KB
-  static constexpr int kStep = 4 * kRows, kScales = 2 * kStep;    // then 4 steps x 256 scales
-  static constexpr int kLds = kScales + 4 * 1024;
+  static constexpr int kStep = 4 * kRows, kScales = 2 * kStep;    // then 4 steps x 256 scales of rows
+  static constexpr int kHeld = kScales + 4 * 1024;                // and each wave's columns' scales of 256 steps
+  static constexpr int kLds = kHeld + 8 * 1024;
 };
 
 template <typename O>
@@ -384,10 +391,12 @@ __global__ __launch_bounds__(512, 2) void k_eight(MatArgs p, int tiles_m, int ti
     w[j][h] = *(const i32x4*)(lw + (k & 1) * Q::kStep + j * 16 * kBlockK + (h ? piece ^ 64 : piece));
   };
 
-  // the columns' scales of 64 steps: one in each lane
+  // the columns' scales of 256 steps in LDS, of 64 of them one in each lane
   const float* sb = (const float*)p.sb + min(n, p.n - 1) / kBlockK * p.sb_pitch;
-  float sbs = sb[min(lane, last)];
-  asm volatile("" : "+v"(sbs));
+  auto load_columns = [&](int k, int i) {
+    load_lds<4>(buffer_of(sb + k), (uint32_t)min(64 * i + lane, last - k) * 4, 0, base + Q::kHeld + wave * 1024 + i * 256);
+  };
+  const float* held = (const float*)(lds + Q::kHeld + wave * 1024) + lane;
 
   f32x4 acc[8][4], t[4];
 #pragma unroll
@@ -395,6 +404,8 @@ __global__ __launch_bounds__(512, 2) void k_eight(MatArgs p, int tiles_m, int ti
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+#pragma unroll
+  for (int i = 0; i < 4; ++i) load_columns(0, i);
   load_s(0), load_s(1);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -405,6 +416,7 @@ __global__ __launch_bounds__(512, 2) void k_eight(MatArgs p, int tiles_m, int ti
     load_s(k + 2);
   }
   meet<12>();
+  float sbs = held[0];
   f32x4 next[2] = {*(const f32x4*)ls, *(const f32x4*)(ls + 16)};
 #pragma unroll
   for (int i = 0; i < 4; ++i) read_x(0, i, 0), read_x(0, i, 1);
@@ -415,8 +427,12 @@ __global__ __launch_bounds__(512, 2) void k_eight(MatArgs p, int tiles_m, int ti
 #pragma unroll 1
   for (int k = 0; k < p.kb; ++k) {
     if ((k & 63) == 0 && k) {
-      sbs = sb[min(k + lane, last)];
-      asm volatile("" : "+v"(sbs));
+      if ((k & 255) == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_columns(k, i);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      sbs = held[k & 192];
     }
     const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sbs), k & 63));
     float s[8];
