@@ -14,7 +14,7 @@
 namespace {
 
 using NormFn = int (*)(int, void*, int, int, int, const void*, int64_t, const void*, int64_t, const void*, void*, void*,
-                       void*, int64_t, int, float);
+                       void*, int64_t, int, double);
 using QuantizeFn = int (*)(int, void*, int, int, int, const void*, int64_t, void*, void*, int64_t, int);
 using MatmulFn = int (*)(int, void*, int, int, const void*, const void*, const void*, const void*, const void*, void*,
                          int64_t, int64_t, int, int64_t, int64_t, void*, int64_t);
@@ -34,14 +34,16 @@ const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariab
 
 bool recorded(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
-// a matrix on a GPU whose columns are neighbours, of a type the operators take, and no part of a graph
+// a matrix on a GPU whose columns are neighbours, of a type the operators take, and no part of a graph (a view that
+// negates its values holds others than it shows)
 bool matrix(const at::Tensor& t) {
   return t.is_cuda() && t.layout() == at::kStrided && t.dim() == 2 && t.size(1) >= 1 &&
-         (t.stride(1) == 1 || t.size(1) == 1) && type_of(t.scalar_type()) >= 0 && !recorded(t);
+         (t.stride(1) == 1 || t.size(1) == 1) && type_of(t.scalar_type()) >= 0 && !t.is_neg() && !recorded(t);
 }
 
 bool neighbours(const at::Tensor& t, int64_t n, const at::Device& device) {
-  return t.device() == device && t.dim() == 1 && t.size(0) == n && (n == 1 || t.stride(0) == 1) && !recorded(t);
+  return t.device() == device && t.layout() == at::kStrided && t.dim() == 1 && t.size(0) == n && (n == 1 || t.stride(0) == 1) &&
+         !t.is_neg() && !recorded(t);
 }
 
 at::Tensor values_for(const at::Tensor& x) {
@@ -62,7 +64,7 @@ bool laid_out(const at::Tensor& v, const at::Tensor& s, const at::Device& device
   if (v.device() != device || s.device() != device || v.scalar_type() != at::kFloat8_e4m3fn || v.dim() != 2 || s.dim() != 2 ||
       v.size(0) != rows || v.size(1) != kb * kBlock || !v.is_contiguous() ||
       (s.scalar_type() != at::kFloat && s.scalar_type() != at::kFloat8_e8m0fnu) ||
-      ((uintptr_t)v.data_ptr() | (uintptr_t)s.data_ptr()) % 16)
+      s.is_neg() || recorded(v) || recorded(s) || ((uintptr_t)v.data_ptr() | (uintptr_t)s.data_ptr()) % 16)
     return false;
   if (tiles) return s.size(0) == (rows + kBlock - 1) / kBlock && s.size(1) == (kb + 3) / 4 * 4 && s.is_contiguous();
   const int64_t pitch = (rows + 7) / 8 * 8;
@@ -90,11 +92,14 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
   if (!(eps >= 0) || cols > (1 << 30)) return refused();
   at::Tensor q = values_for(*x), s = scales_for(*x, false, pow2), h;
   if (r) h = at::empty({rows, cols}, x->options());
+  // (what may throw comes before the lock is given up)
+  const int device = x->get_device(), type = type_of(x->scalar_type());
+  const int64_t pitch = x->stride(0), r_pitch = r ? r->stride(0) : 0;
+  const void *from = x->data_ptr(), *add = r ? r->data_ptr() : nullptr, *by = w->data_ptr();
+  void *sum = r ? h.data_ptr() : nullptr, *values = q.data_ptr(), *scales = s.data_ptr();
   int rc = 0;
   Py_BEGIN_ALLOW_THREADS
-  rc = norm_entry(x->get_device(), stream, type_of(x->scalar_type()), wide, pow2 != 0, x->data_ptr(), x->stride(0),
-                  r ? r->data_ptr() : nullptr, r ? r->stride(0) : 0, w->data_ptr(), r ? h.data_ptr() : nullptr, q.data_ptr(),
-                  s.data_ptr(), rows, (int)cols, (float)eps);
+  rc = norm_entry(device, stream, type, wide, pow2 != 0, from, pitch, add, r_pitch, by, sum, values, scales, rows, (int)cols, eps);
   Py_END_ALLOW_THREADS
   if (rc) return PyLong_FromLong(rc);
   PyObject* out = PyTuple_New(3);
@@ -120,10 +125,13 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t count) {
   void* stream = PyLong_AsVoidPtr(args[3]);
   if (PyErr_Occurred()) return nullptr;
   at::Tensor q = values_for(*x), s = scales_for(*x, tiles, pow2);
+  const int device = x->get_device(), type = type_of(x->scalar_type());
+  const int64_t pitch = x->stride(0), rows = x->size(0), cols = x->size(1);
+  const void* from = x->data_ptr();
+  void *values = q.data_ptr(), *scales = s.data_ptr();
   int rc = 0;
   Py_BEGIN_ALLOW_THREADS
-  rc = quantize_entry(x->get_device(), stream, type_of(x->scalar_type()), tiles != 0, pow2 != 0, x->data_ptr(), x->stride(0),
-                      q.data_ptr(), s.data_ptr(), x->size(0), (int)x->size(1));
+  rc = quantize_entry(device, stream, type, tiles != 0, pow2 != 0, from, pitch, values, scales, rows, (int)cols);
   Py_END_ALLOW_THREADS
   if (rc) return PyLong_FromLong(rc);
   PyObject* out = PyTuple_New(2);
@@ -157,8 +165,9 @@ PyObject* matmul(PyObject*, PyObject* const* args, Py_ssize_t count) {
     out = *given;
     if (!out.is_cuda() || out.layout() != at::kStrided || out.dim() != 2 || out.scalar_type() != out_type ||
         out.device() != device || out.size(0) != m || out.size(1) != n || (n > 1 && out.stride(1) != 1) ||
-        (m > 1 && out.stride(0) < n) || recorded(out))
+        (m > 1 && out.stride(0) < n) || out.is_neg() || recorded(out))
       return refused();
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();        // written in place
   } else {
     out = at::empty({m, n}, a->options().dtype(out_type));
   }
@@ -166,11 +175,13 @@ PyObject* matmul(PyObject*, PyObject* const* args, Py_ssize_t count) {
   const int64_t bytes = workspace_entry(m, n, kb, pow2);
   at::Tensor room;
   if (bytes) room = at::empty({bytes}, a->options().dtype(at::kByte));
+  const int64_t pitch = m > 1 ? out.stride(0) : std::max<int64_t>(n, 1);
+  const void *pa = a->data_ptr(), *psa = sa->data_ptr(), *pb = b->data_ptr(), *psb = sb->data_ptr(),
+             *add = bias ? bias->data_ptr() : nullptr;
+  void *to = out.data_ptr(), *space = bytes ? room.data_ptr() : nullptr;
   int rc = 0;
   Py_BEGIN_ALLOW_THREADS
-  rc = matmul_entry(device.index(), stream, (int)type, pow2, a->data_ptr(), sa->data_ptr(), b->data_ptr(), sb->data_ptr(),
-                    bias ? bias->data_ptr() : nullptr, out.data_ptr(), m, n, kb, m > 1 ? out.stride(0) : std::max<int64_t>(n, 1),
-                    (m + 7) / 8 * 8, bytes ? room.data_ptr() : nullptr, bytes);
+  rc = matmul_entry(device.index(), stream, (int)type, pow2, pa, psa, pb, psb, add, to, m, n, kb, pitch, (m + 7) / 8 * 8, space, bytes);
   Py_END_ALLOW_THREADS
   if (rc) return PyLong_FromLong(rc);
   return THPVariable_Wrap(std::move(out));

@@ -151,7 +151,7 @@ struct NormArgs {
   void *stream_out, *values, *scales;
   int64_t rows, x_pitch, r_pitch, s_pitch;   // pitches in elements
   int cols, padded;
-  float eps;
+  double eps;
 };
 
 // One workgroup a row. CHUNKS > 0: the row stays in registers (padded <= THREADS * CHUNKS * 8);
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
   };
 
   float kept[CHUNKS ? CHUNKS : 1][kWidth];
-  float sum = 0.f;
+  double sum = 0.;
 #pragma unroll
   for (int k = 0; k < chunks; ++k) {
     const int c = (k * THREADS + tid) * kWidth;
@@ -189,14 +189,14 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
     if (c < a.padded) {
       take(c, h);
 #pragma unroll
-      for (int i = 0; i < kWidth; ++i) sum = fmaf(h[i], h[i], sum);
+      for (int i = 0; i < kWidth; ++i) sum = fma((double)h[i], (double)h[i], sum);
     } else {
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) h[i] = 0.f;
     }
   }
-  // a lane's squares are summed in float32, the lanes' sums and the root are taken in 64 bits
-  double total = wave_sum((double)sum);
+  // squares, sums and the root in 64 bits: float32 would lose rows below 1e-19 and above 1e19, and it takes no longer
+  double total = wave_sum(sum);
   if constexpr (kWaves > 1) {
     if ((tid & 63) == 0) part[tid >> 6] = total;
     __syncthreads();
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
         gmax = fmaxf(gmax, finite_abs(g[i]));
       }
       gmax = row_max(gmax);
-      float amax = rstd == rstd ? fminf(gmax * rstd, 3.402823466e38f) : 0.f;   // a NaN in the row: NaN values, scale 1
+      float amax = rstd <= 3.402823466e38f ? fminf(gmax * rstd, 3.402823466e38f) : 0.f;   // NaN in the row, or 1/0: NaN, scale 1
       // a product that was rounded down onto 448 * 2^p lies above it
       if (POW2 && fmaf(gmax, rstd, -amax) + gmax * rstd_low > 0.f && amax < 3.4e38f)
         amax = __uint_as_float(__float_as_uint(amax) + 1);
@@ -331,8 +331,11 @@ __global__ __launch_bounds__(kThreads) void k_tiles(QuantArgs a) {
 
 int padded_cols(int cols) { return (cols + kBlockK - 1) / kBlockK * kBlockK; }
 
+// A launch holds fewer than 2^32 threads, so a matrix goes in pieces of at most this many rows.
+constexpr int64_t kRowsALaunch = 1 << 21;
+
 template <typename T, typename W, bool POW2, bool RES>
-int norm_sized(const NormArgs& a, hipStream_t s) {
+int norm_piece(const NormArgs& a, hipStream_t s) {
   const unsigned grid = (unsigned)((a.rows + kXcds - 1) / kXcds * kXcds);
 #define YODA_NORM(threads, chunks) k_norm<T, W, POW2, RES, threads, chunks><<<grid, threads, 0, s>>>(a)
   if (a.padded <= 64 * 8) YODA_NORM(64, 1);
@@ -347,6 +350,21 @@ int norm_sized(const NormArgs& a, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
+template <typename T, typename W, bool POW2, bool RES>
+int norm_sized(const NormArgs& all, hipStream_t s) {
+  int rc = 0;
+  for (int64_t at = 0; at < all.rows && !rc; at += kRowsALaunch) {
+    NormArgs a = all;
+    a.rows = all.rows - at < kRowsALaunch ? all.rows - at : kRowsALaunch;
+    a.x = (const T*)all.x + at * all.x_pitch;
+    if (RES) a.residual = (const T*)all.residual + at * all.r_pitch, a.stream_out = (T*)all.stream_out + at * all.cols;
+    a.values = (uint8_t*)all.values + at * all.padded;
+    a.scales = (uint8_t*)all.scales + at * (POW2 ? 1 : 4);
+    rc = norm_piece<T, W, POW2, RES>(a, s);
+  }
+  return rc;
+}
+
 template <typename T, typename W>
 int norm_typed(const NormArgs& a, bool pow2, hipStream_t s) {
   if (pow2) return a.residual ? norm_sized<T, W, true, true>(a, s) : norm_sized<T, W, true, false>(a, s);
@@ -354,18 +372,24 @@ int norm_typed(const NormArgs& a, bool pow2, hipStream_t s) {
 }
 
 template <typename T>
-int quant_typed(const QuantArgs& a, bool tiles, bool pow2, hipStream_t s) {
+int quant_typed(const QuantArgs& all, bool tiles, bool pow2, hipStream_t s) {
   if (tiles) {
-    const int64_t grid = (a.rows + kBlockK - 1) / kBlockK * (a.padded / kBlockK);
-    if (grid > 0x7FFFFFFF) return -1;
-    if (pow2) k_tiles<T, true><<<(unsigned)grid, kThreads, 0, s>>>(a);
-    else k_tiles<T, false><<<(unsigned)grid, kThreads, 0, s>>>(a);
+    const int64_t grid = (all.rows + kBlockK - 1) / kBlockK * (all.padded / kBlockK);
+    if (grid >= 1 << 24) return -1;             // 2^32 threads; 256 GB of values
+    if (pow2) k_tiles<T, true><<<(unsigned)grid, kThreads, 0, s>>>(all);
+    else k_tiles<T, false><<<(unsigned)grid, kThreads, 0, s>>>(all);
   } else {
-    const int64_t per = kThreads >> a.lane_bits, count = (a.rows + per - 1) / per;
-    const int64_t grid = (count + kXcds - 1) / kXcds * kXcds;
-    if (grid > 0x7FFFFFFF) return -1;
-    if (pow2) k_rows<T, true><<<(unsigned)grid, kThreads, 0, s>>>(a);
-    else k_rows<T, false><<<(unsigned)grid, kThreads, 0, s>>>(a);
+    for (int64_t at = 0; at < all.rows; at += kRowsALaunch) {
+      QuantArgs a = all;
+      a.rows = all.rows - at < kRowsALaunch ? all.rows - at : kRowsALaunch;
+      a.x = (const T*)all.x + at * all.pitch;
+      a.values = (uint8_t*)all.values + at * all.padded;
+      a.scales = (uint8_t*)all.scales + at * (pow2 ? 1 : 4);
+      const int64_t per = kThreads >> a.lane_bits, count = (a.rows + per - 1) / per;
+      const unsigned grid = (unsigned)((count + kXcds - 1) / kXcds * kXcds);
+      if (pow2) k_rows<T, true><<<grid, kThreads, 0, s>>>(a);
+      else k_rows<T, false><<<grid, kThreads, 0, s>>>(a);
+    }
   }
   return (int)hipGetLastError();
 }
@@ -382,7 +406,7 @@ extern "C" {
 // Returns 0, a hipError, or -1 for arguments out of range.
 int yoda_fp8_norm(int device, void* stream, int type, int weight_f32, int pow2, const void* x, int64_t x_pitch,
                   const void* residual, int64_t r_pitch, const void* weight, void* stream_out, void* values,
-                  void* scales, int64_t rows, int cols, float eps) {
+                  void* scales, int64_t rows, int cols, double eps) {
   if (!valid_type(type) || rows < 0 || rows > 0x7FFFFF00 || cols < 1 || cols > (1 << 30)) return -1;
   if ((residual == nullptr) != (stream_out == nullptr)) return -1;
   if (rows == 0) return 0;

@@ -21,6 +21,9 @@ struct MatArgs {
   int kb, sb_pitch;                    // Kp / 128, and up to a multiple of 4
 };
 
+// A launch holds fewer than 2^32 threads, 512 of them a workgroup at most.
+constexpr int64_t kMostGroups = 1 << 22;
+
 template <int I>
 struct Index {
   static constexpr int value = I;
@@ -480,7 +483,7 @@ __global__ __launch_bounds__(512, 2) void k_eight(MatArgs p, int tiles_m, int ti
 template <typename O>
 int run_256(const MatArgs& p, bool pow2, hipStream_t s) {
   const int64_t tm = (p.m + 255) / 256, tn = (p.n + 255) / 256, total = tm * tn;
-  if (total > (1 << 30)) return -1;
+  if (total >= kMostGroups) return -1;          // 512 GB of output
   const unsigned grid = (unsigned)((total + 7) / 8 * 8);
   if (pow2) k_quarters<O><<<grid, 256, 0, s>>>(p, (int)tm, (int)tn);
   else k_eight<O><<<grid, 512, 0, s>>>(p, (int)tm, (int)tn);
@@ -709,7 +712,6 @@ template <int RP, int CP, int STAGES, typename O>
 int run_mid(const MatArgs& p, bool pow2, int count, float* parts, hipStream_t s) {
   using Q = Mid<RP, CP>;
   const int64_t tm = (p.m + Q::BM - 1) / Q::BM, tn = (p.n + Q::BN - 1) / Q::BN, total = tm * tn;
-  if (total > (1 << 26) || count > 65535) return -1;
   const dim3 grid((unsigned)((total + 7) / 8 * 8), count);
   float* to = count > 1 ? parts : nullptr;
   if (pow2) k_mid<RP, CP, STAGES, O, true><<<grid, 256, STAGES * Q::kStage, s>>>(p, (int)tm, (int)tn, to);
@@ -724,24 +726,22 @@ int run_mid(const MatArgs& p, bool pow2, int count, float* parts, hipStream_t s)
 // take every WAVES-th block of K and read their operands from memory straight into registers, DEPTH
 // blocks ahead, each weight byte once on the whole card; the rows are read again by each workgroup, out of L2.
 // No wave waits for another until the end, when the waves' sums are added through LDS in the order of
-// the waves. Rows m = c * MP + i as in the tiles; columns as in column_of where NP is 2.
-template <int MP, int NP, int WAVES, int DEPTH, typename O, bool POW2>
+// the waves. Lane (c, g) has row c; columns as in column_of where NP is 2.
+template <int NP, int WAVES, int DEPTH, typename O, bool POW2>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_narrow(MatArgs p) {
-  __shared__ f32x4 part[WAVES * MP * NP * 64];
+  __shared__ f32x4 part[WAVES * NP * 64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16 * NP, kp = (int64_t)p.kb * kBlockK;
-  const uint8_t *px[MP], *pw[NP];
-#pragma unroll
-  for (int i = 0; i < MP; ++i) px[i] = p.a + min((int64_t)c * MP + i, p.m - 1) * kp + g * 16;
+  const uint8_t *px = p.a + min((int64_t)c, p.m - 1) * kp + g * 16, *pw[NP];
 #pragma unroll
   for (int j = 0; j < NP; ++j) pw[j] = p.b + min(n0 + (NP == 2 ? column_of(j, c) : c), p.n - 1) * kp + g * 16;
-  const int64_t sa_at = min((int64_t)c * MP, p.sa_pitch - MP), sb_at = n0 / kBlockK * p.sb_pitch;
+  const int64_t sa_at = min((int64_t)c, p.sa_pitch - 1), sb_at = n0 / kBlockK * p.sb_pitch;
 
   struct Block {
-    i32x4 x[MP][2], w[NP][2];
-    float xs[MP], ws;
-    uint32_t xb[MP > 4 ? 2 : 1], wb;
+    i32x4 x[2], w[NP][2];
+    float xs, ws;
+    uint32_t xb, wb;
   };
   auto load = [&](Block& b, int kb) {
     const int64_t at = (int64_t)kb * kBlockK;
@@ -750,46 +750,33 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_narrow(MatArgs p) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) b.w[j][h] = *(const i32x4*)(pw[j] + at + 64 * h);
 #pragma unroll
-    for (int i = 0; i < MP; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) b.x[i][h] = *(const i32x4*)(px[i] + at + 64 * h);
+    for (int h = 0; h < 2; ++h) b.x[h] = *(const i32x4*)(px + at + 64 * h);
     const int64_t s = kb * p.sa_pitch + sa_at;
     if constexpr (POW2) {
-      const uint8_t* q = (const uint8_t*)p.sa + s;
-      if constexpr (MP == 1) b.xb[0] = *q;
-      else if constexpr (MP == 2) b.xb[0] = *(const uint16_t*)q;
-      else if constexpr (MP == 4) b.xb[0] = *(const uint32_t*)q;
-      else b.xb[0] = ((const uint32_t*)q)[0], b.xb[1] = ((const uint32_t*)q)[1];
+      b.xb = ((const uint8_t*)p.sa)[s];
       b.wb = ((const uint8_t*)p.sb)[sb_at + kb];
     } else {
-#pragma unroll
-      for (int i = 0; i < MP; ++i) b.xs[i] = ((const float*)p.sa)[s + i];
+      b.xs = ((const float*)p.sa)[s];
       b.ws = ((const float*)p.sb)[sb_at + kb];
     }
   };
 
-  f32x4 acc[MP][NP];
+  f32x4 acc[NP];
 #pragma unroll
-  for (int i = 0; i < MP; ++i)
-#pragma unroll
-    for (int j = 0; j < NP; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < NP; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto use = [&](const Block& b) {
-    auto piece = [&](auto I) {
-      constexpr int i = decltype(I)::value;
 #pragma unroll
-      for (int j = 0; j < NP; ++j) {
-        if constexpr (POW2) {
-          acc[i][j] = mfma_scaled<i & 3>(join(b.w[j]), join(b.x[i]), acc[i][j], b.wb, b.xb[i >> 2]);
-        } else {
-          const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-          const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(b.w[j]), join(b.x[i]), zero, 0, 0, 0, 0, 0, 0);
-          const float s = b.xs[i] * b.ws;
+    for (int j = 0; j < NP; ++j) {
+      if constexpr (POW2) {
+        acc[j] = mfma_scaled<0>(join(b.w[j]), join(b.x), acc[j], b.wb, b.xb);
+      } else {
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(b.w[j]), join(b.x), zero, 0, 0, 0, 0, 0, 0);
+        const float s = b.xs * b.ws;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[r], s, acc[i][j][r]);
-        }
+        for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(t[r], s, acc[j][r]);
       }
-    };
-    each<MP>(piece);
+    }
   };
 
   // Rows a power of two apart lie on one memory channel, so workgroups that walk K in step would ask few
@@ -825,26 +812,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_narrow(MatArgs p) {
     if (q + (d + DEPTH) * WAVES < p.kb) use(ring[d]);
 
 #pragma unroll
-  for (int i = 0; i < MP; ++i)
-#pragma unroll
-    for (int j = 0; j < NP; ++j) part[(wave * MP * NP + i * NP + j) * 64 + lane] = acc[i][j];
+  for (int j = 0; j < NP; ++j) part[(wave * NP + j) * 64 + lane] = acc[j];
   __syncthreads();
-  for (int e = threadIdx.x; e < MP * NP * 64; e += 64 * WAVES) {
+  for (int e = threadIdx.x; e < NP * 64; e += 64 * WAVES) {
     f32x4 v = part[e];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) v += part[w * MP * NP * 64 + e];
-    const int l = e & 63, i = e / 64 / NP, j = e / 64 % NP;
-    const int64_t m = (int64_t)(l & 15) * MP + i, n = n0 + (NP == 2 ? (l >> 4) * 8 + j * 4 : (l >> 4) * 4);
+    for (int w = 1; w < WAVES; ++w) v += part[w * NP * 64 + e];
+    const int l = e & 63, j = e / 64;
+    const int64_t m = l & 15, n = n0 + (NP == 2 ? (l >> 4) * 8 + j * 4 : (l >> 4) * 4);
     if (m < p.m && n < p.n) store4<O>(p, v, m, n);
   }
 }
 
-template <int MP, int NP, int WAVES, int DEPTH, typename O>
+template <int NP, int WAVES, int DEPTH, typename O>
 int narrow(const MatArgs& p, bool pow2, hipStream_t s) {
-  const int64_t grid = (p.n + 16 * NP - 1) / (16 * NP);
-  if (grid > 0x7FFFFFFF) return -1;
-  if (pow2) k_narrow<MP, NP, WAVES, DEPTH, O, true><<<(unsigned)grid, 64 * WAVES, 0, s>>>(p);
-  else k_narrow<MP, NP, WAVES, DEPTH, O, false><<<(unsigned)grid, 64 * WAVES, 0, s>>>(p);
+  const unsigned grid = (unsigned)((p.n + 16 * NP - 1) / (16 * NP));
+  if (pow2) k_narrow<NP, WAVES, DEPTH, O, true><<<grid, 64 * WAVES, 0, s>>>(p);
+  else k_narrow<NP, WAVES, DEPTH, O, false><<<grid, 64 * WAVES, 0, s>>>(p);
   return (int)hipGetLastError();
 }
 
@@ -883,7 +867,7 @@ Plan plan(int64_t m, int64_t n, int kb, bool pow2) {
   const int64_t big = (m + 255) / 256 * ((n + 255) / 256);
   const double rest = big % 256 ? (1 + big % 256 / 256.0) / 2 : 0;
   double least = std::max<double>(big / 256 + rest, 1) * (10.5 + kb * (pow2 ? 1.4 : 1.57));
-  if (m <= 16) {
+  if (m <= 16 && n < kMostGroups * 32) {
     const double t = 2 + weight * 1.5 / 8e6 + 3. * ((n + 8191) / 8192 - 1);
     if (t < least) least = t, best = {Plan::kNarrow, 0, 1, 0, 0};
   }
@@ -892,7 +876,7 @@ Plan plan(int64_t m, int64_t n, int kb, bool pow2) {
     const int64_t tiles = (m + 32 * h.rows - 1) / (32 * h.rows) * ((n + 32 * h.columns - 1) / (32 * h.columns));
     for (int parts = 1; parts <= 16 && parts * 2 <= std::max(kb, 2); parts *= 2) {
       const int64_t groups = tiles * parts, bytes = parts > 1 ? groups * h.rows * h.columns * 4096 : 0;
-      if (parts > 1 && groups > 512) break;
+      if ((parts > 1 && groups > 512) || groups >= kMostGroups) break;
       const int steps = (kb + parts - 1) / parts;
       const double rounds = (double)((groups + 511) / 512);
       double t = groups <= 256 ? 5 + steps * (pow2 ? h.one : h.one_f) : 2 + rounds * (h.round + steps * (pow2 ? h.two : h.two_f));
@@ -910,7 +894,7 @@ int run(const MatArgs& p, bool pow2, float* workspace, int64_t bytes, hipStream_
   if (to.bytes > bytes || (to.bytes && !workspace)) return -1;
   if (to.kind == Plan::k256) return run_256<O>(p, pow2, s);
   // two pieces of columns a workgroup halve what is read of the rows, where that leaves enough workgroups
-  if (to.kind == Plan::kNarrow) return p.n >= 8192 ? narrow<1, 2, 8, 4, O>(p, pow2, s) : narrow<1, 1, 8, 4, O>(p, pow2, s);
+  if (to.kind == Plan::kNarrow) return p.n >= 8192 ? narrow<2, 8, 4, O>(p, pow2, s) : narrow<1, 8, 4, O>(p, pow2, s);
   // stages: those of one workgroup fill LDS where there is one on a CU, else those of two
   const bool alone = to.groups <= 256;
   if (to.shape == 0) return alone ? run_mid<4, 4, 4, O>(p, pow2, to.parts, workspace, s) : run_mid<4, 4, 2, O>(p, pow2, to.parts, workspace, s);

@@ -12,7 +12,7 @@
 extern "C" {
 int yoda_fp8_norm(int device, void* stream, int type, int weight_f32, int pow2, const void* x, int64_t x_pitch,
                   const void* residual, int64_t r_pitch, const void* weight, void* stream_out, void* values,
-                  void* scales, int64_t rows, int cols, float eps);
+                  void* scales, int64_t rows, int cols, double eps);
 int yoda_fp8_quantize(int device, void* stream, int type, int tiles, int pow2, const void* x, int64_t pitch,
                       void* values, void* scales, int64_t rows, int cols);
 int64_t yoda_fp8_matmul_workspace(int64_t m, int64_t n, int kb, int pow2);
@@ -24,7 +24,7 @@ int yoda_fp8_matmul(int device, void* stream, int out_type, int pow2, const void
 namespace yoda_fp8 {
 namespace {
 
-constexpr float kEps = 1e-6f;
+constexpr double kEps = 1e-6;
 
 // about normal (a sum of four uniform values), from the element's place and the seed; bf16
 __global__ __launch_bounds__(256) void k_values(uint16_t* out, int64_t n, uint32_t seed, float scale, float shift) {
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(128) void k_check_norm(const uint16_t* x, const uin
   __syncthreads();
   const float v = (float)bf16(x, m * cols + c) + (float)bf16(r, m * cols + c);
   const uint16_t hb = store_bits<__hip_bfloat16>(v);
-  const double y = (double)load_f32<__hip_bfloat16>(hb) / sqrt(sum / cols + (double)kEps) * bf16(gain, c);
+  const double y = (double)load_f32<__hip_bfloat16>(hb) / sqrt(sum / cols + kEps) * bf16(gain, c);
   part[t] = fabs(y);
   __syncthreads();
   double amax = 0;

@@ -86,6 +86,23 @@ def test_matmul_refuses(a, b, kw, error):
         fp8.matmul(a, b, **kw)
 
 
+def test_what_is_no_plain_tensor_is_refused():
+    x = torch.ones(4, 128)
+    for bad, error in ((None, TypeError), ([1.0], TypeError), (torch._neg_view(x), ValueError), (x.to_sparse(), ValueError)):
+        with pytest.raises(error):
+            fp8._refuse_matrix(bad, "x")
+
+
+def test_scales_that_are_learned_are_refused():
+    """A block matrix takes them; a product that would lose their gradient does not."""
+    b = fp8.BlockMatrix(torch.zeros(4, 128).to(E4M3), torch.ones(1, 1, requires_grad=True), block_rows=128)
+    a = _matrix(4, 128)
+    with pytest.raises(RuntimeError, match="backward"):
+        fp8.matmul(a, b)
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+        fp8.matmul(a, b)
+
+
 class FakeProber:
     """A node's probes without a GPU: HIP ordinal d is amd-smi index d."""
 

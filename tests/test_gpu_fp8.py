@@ -482,6 +482,79 @@ def test_offsets_past_32_bits(require_gpu, m):
 
 
 @pytest.mark.parametrize("pow2", [False, True])
+def test_norm_of_small_and_large_rows(require_gpu, pow2):
+    """Squares that float32 does not hold, an eps that it does not hold, and a root that nothing holds."""
+    fp8 = _ops()
+    x = _randn((6, 640), 77).double()
+    x[0] *= 2.0 ** -90
+    x[1] *= 2.0 ** 100
+    x[2] *= 2.0 ** -64
+    x[4:] = 0
+    x, w = x.float(), torch.ones(640)
+    sd = E8M0 if pow2 else torch.float32
+    q, h = fp8.add_rms_norm(x[:4].to(DEV), w.to(DEV), None, 0.0, sd)
+    _check_norm(q, h, x[:4], w, None, 0.0, pow2)
+    q, h = fp8.add_rms_norm(x[:5].to(DEV), w.to(DEV), None, 1e-60, sd)
+    _check_norm(q, h, x[:5], w, None, 1e-60, pow2)
+    q, _ = fp8.add_rms_norm(x[4:].to(DEV), w.to(DEV), None, 0.0, sd)
+    assert q.values.float().isnan().all() and (q.scales.float() == 1).all()
+
+
+@pytest.mark.parametrize("pow2", [False, True])
+def test_more_rows_than_a_launch_takes(require_gpu, pow2):
+    fp8 = _ops()
+    sd = E8M0 if pow2 else torch.float32
+    rows, cut = (1 << 21) + 13, (1 << 21) - 5
+    g = torch.Generator(DEV).manual_seed(5)
+    x, r = (torch.randn(rows, 40, generator=g, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    w = torch.randn(40, generator=g, device=DEV, dtype=torch.bfloat16)
+    for all_, end, start in ((fp8.quantize(x, 1, sd), fp8.quantize(x[cut:], 1, sd), fp8.quantize(x[:40], 1, sd)),
+                             tuple(fp8.add_rms_norm(a, w, b, 1e-6, sd)[0]
+                                   for a, b in ((x, r), (x[cut:], r[cut:]), (x[:40], r[:40])))):
+        for part, piece in ((slice(cut, None), end), (slice(0, 40), start)):
+            assert torch.equal(all_.data[part].view(torch.uint8), piece.data.view(torch.uint8))
+            assert torch.equal(all_.scales.float()[part], piece.scales.float())
+    h = fp8.add_rms_norm(x, w, r)[1]
+    assert torch.equal(h, (x.float() + r.float()).to(x.dtype))
+
+
+@pytest.mark.parametrize("m", [2, 20])
+def test_more_columns_than_a_launch_takes(require_gpu, m):
+    """2^27 columns of 32 a workgroup: the choice goes to larger tiles."""
+    fp8 = _ops()
+    n = (1 << 27) + 70
+    g = torch.Generator(DEV).manual_seed(6)
+    values = torch.randint(0, 0x60, (n, 128), dtype=torch.uint8, device=DEV, generator=g).view(E4M3)
+    scales = torch.rand(-(-n // 128), 1, device=DEV, generator=g)
+    a = fp8.quantize(torch.randn(m, 128, device=DEV, generator=g))
+    out = fp8.matmul(a, fp8.BlockMatrix(values, scales, block_rows=128))
+    for first in (0, (1 << 26), n - 70 - 128):
+        first = first // 128 * 128
+        part = fp8.BlockMatrix(values[first:first + 198], scales[first // 128:first // 128 + -(-len(values[first:first + 198]) // 128)],
+                               block_rows=128)
+        want = _dequantized(a) @ _dequantized(part).T
+        got = out[:, first:first + want.shape[1]].cpu().double()
+        mass = _dequantized(a).abs() @ _dequantized(part).abs().T
+        assert ((got - want).abs() <= mass * (7 * 2.0 ** -13 + 256 * 2.0 ** -24) + want.abs() * 2.0 ** -8).all()
+
+
+def test_out_counts_as_written(require_gpu):
+    fp8 = _ops()
+    a, b = fp8.quantize(torch.ones(4, 128, device=DEV)), fp8.quantize(torch.ones(8, 128, device=DEV), 128)
+    out = torch.empty(4, 8, device=DEV, dtype=torch.bfloat16)
+    before = out._version
+    assert fp8.matmul(a, b, out=out) is out and out._version > before
+    with torch.inference_mode():
+        assert (fp8.matmul(a, b, out=torch.empty_like(out)) == 128).all()
+    learned = fp8.BlockMatrix(b.values, b.scales.clone().requires_grad_(), block_rows=128)
+    with pytest.raises(RuntimeError):
+        fp8.matmul(a, learned)
+    for x in (torch._neg_view(torch.ones(4, 128, device=DEV)), torch.ones(4, 128, device=DEV).to_sparse()):
+        with pytest.raises(ValueError):
+            fp8.quantize(x)
+
+
+@pytest.mark.parametrize("pow2", [False, True])
 @pytest.mark.parametrize("rows,cols,inner", [(1, 256, 128), (37, 512, 384), (300, 768, 1024), (1, 8192, 2048)])
 def test_matrix_check_is_clean(require_gpu, rows, cols, inner, pow2):
     from yoda_scheduler_amd.ops import hip

@@ -152,6 +152,7 @@ def _stream_of(x: torch.Tensor) -> int:
 
 
 def _refuse_matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None) -> None:
+    _refuse_other(t, name)
     if t.dim() != 2 or t.stride(1) != 1 and t.shape[1] > 1:
         raise ValueError(f"{name}: a 2-D tensor whose columns are neighbours, not {tuple(t.shape)} "
                          f"with strides {t.stride()}")
@@ -162,6 +163,13 @@ def _refuse_matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = No
     if not t.is_cuda:
         raise ValueError(f"{name} is on {t.device}: these operators run on a GPU")
     _no_grad(t)
+
+
+def _refuse_other(t: torch.Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a tensor, not {type(t).__name__}")
+    if t.layout != torch.strided or t.is_neg():
+        raise ValueError(f"{name}: a plain tensor, neither sparse nor a negated view")
 
 
 def _no_grad(*tensors: Optional[torch.Tensor]) -> None:
@@ -205,7 +213,9 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
 
     Returns (y in e4m3 with 1 × 128 blocks, h); h is None without a residual. ``weight`` [cols] has
     x's type or is float32; x and residual [rows, cols] may have any row stride. Values are the 8-bit ones next to
-    the quotients themselves. A row that holds NaN is NaN; squares are summed in float32.
+    the quotients themselves. Squares are summed in 64 bits, the rest is float32: it holds for rows whose
+    root mean square and products h * weight lie between 2^-100 and 2^120. A row that holds NaN is NaN, and so is
+    one of zeros where eps is 0.
     """
     pow2 = _scale_kind(scale_dtype)
     got = _native().norm(x, weight, residual, eps, pow2, _stream_of(x))
@@ -218,6 +228,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     rows, cols = x.shape
     if not eps >= 0:
         raise ValueError(f"eps: 0 or more, not {eps}")
+    _refuse_other(weight, "weight")
     if weight.shape != (cols,) or cols > 1 and weight.stride(0) != 1:
         raise ValueError(f"weight: {cols} neighbouring values, not {tuple(weight.shape)} with strides {weight.stride()}")
     if weight.dtype != x.dtype and weight.dtype != torch.float32:
@@ -241,7 +252,8 @@ def matmul(a: BlockMatrix, b: BlockMatrix, out_dtype: torch.dtype = torch.bfloat
 
     The matrix instruction adds eight neighbouring products in fixed point, cutting each off at 2^-13
     of the largest, before they reach the float32 sum: about 2^-16 of a result, well below a 16-bit
-    output's own rounding and short of float32's, so there is no float32 output. The order of the sums goes
+    output's own rounding and short of float32's, so there is no float32 output. Float32 scales of a and b are
+    multiplied first, so their products have to lie between 2^-126 and 2^127. The order of the sums goes
     by the sizes alone: the same call gives the same bits, and another number of rows may not.
     """
     kind = _OUT.get(out_dtype)
@@ -255,6 +267,7 @@ def matmul(a: BlockMatrix, b: BlockMatrix, out_dtype: torch.dtype = torch.bfloat
         raise ValueError(f"a has blocks of {a.block_rows} row(s) and b of {b.block_rows}: 1 and {BLOCK} are wanted")
     if a.cols != b.cols:
         raise ValueError(f"a has {a.cols} columns, b {b.cols}")
+    _no_grad(a.data, a._room, b.data, b._room)
     if a._room.dtype != b._room.dtype:
         raise TypeError(f"a's scales are {a._room.dtype}, b's {b._room.dtype}")
     device = a.data.device
@@ -266,12 +279,14 @@ def matmul(a: BlockMatrix, b: BlockMatrix, out_dtype: torch.dtype = torch.bfloat
         raise TypeError(f"out_dtype: bfloat16 or float16, not {out_dtype}")
     m, n = a.rows, b.rows
     if bias is not None:
+        _refuse_other(bias, "bias")
         if bias.dtype != out_dtype:
             raise TypeError(f"bias: {out_dtype}, not {bias.dtype}")
         if bias.shape != (n,) or n > 1 and bias.stride(0) != 1 or bias.device != device:
             raise ValueError(f"bias: {n} neighbouring values on {device}, not {tuple(bias.shape)} on {bias.device}")
         _no_grad(bias)
     if out is not None:
+        _refuse_other(out, "out")
         if out.shape != (m, n) or out.device != device or m > 1 and out.stride(0) < n:
             raise ValueError(f"out: {(m, n)} on {device} with rows apart, not {tuple(out.shape)} on {out.device} "
                              f"with strides {out.stride()}")

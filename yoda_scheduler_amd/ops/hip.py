@@ -45,7 +45,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "yoda_hip_occupy_wait": [c_int],
         # ops/fp8.py: device, stream, types and switches, tensors, sizes
         "yoda_fp8_norm": [c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-                          c_void_p, c_void_p, c_void_p, c_int64, c_int, c_float],
+                          c_void_p, c_void_p, c_void_p, c_int64, c_int, c_double],
         "yoda_fp8_quantize": [c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
                               c_int],
         "yoda_fp8_matmul": [c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
