@@ -156,6 +156,12 @@ struct NormArgs {
 
 // One workgroup a row. CHUNKS > 0: the row stays in registers (padded <= THREADS * CHUNKS * 8);
 // CHUNKS == 0: the row is read twice (rows wider than that).
+//
+// Many rows: HBM. 16384 x 8192 in bf16 with a residual stream moves 940 MB in 186 us, 5.05 TB/s where a copy of 1 GB
+// reaches 5.12; 512 or 1024 lanes a row, non-temporal loads and stores, and 32-bit sums were no faster.
+// Few rows: the way of one row through load, sum, barrier, weight and store. Twice the lanes take
+// 1 x 4096 from 4.5 to 3.6 us, 333 x 5001 from 6.4 to 5.6 and 64 x 8192 from 7.3 to 5.1 up to 1024 rows
+// (four a CU); with more they cost 3 % (4096 x 4096 30.7 : 31.3) to 5 % (2000 x 5001 14.6 : 15.3).
 template <typename T, typename W, bool POW2, bool RES, int THREADS, int CHUNKS>
 __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
   constexpr int kWaves = THREADS / 64;
@@ -180,13 +186,16 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
     }
   };
 
-  float kept[CHUNKS ? CHUNKS : 1][kWidth];
+  // one chunk a lane: the weight is asked for with the row, not after the sum (1024 x 4096 10.3 -> 9.8 us)
+  constexpr bool kEarly = CHUNKS == 1;
+  float kept[CHUNKS ? CHUNKS : 1][kWidth], early[kWidth];
   double sum = 0.;
 #pragma unroll
   for (int k = 0; k < chunks; ++k) {
     const int c = (k * THREADS + tid) * kWidth;
     float(&h)[kWidth] = kept[CHUNKS ? k : 0];
     if (c < a.padded) {
+      if constexpr (kEarly) load8<W>(w, c, a.cols, early);
       take(c, h);
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) sum = fma((double)h[i], (double)h[i], sum);
@@ -220,8 +229,9 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
       //   y / s = 448 g / max |g|,  or for a power of two  y / s = g * (rstd / s),
       // each with its first rounding's error added back and rounded to odd: the conversion that follows then
       // gives the 8-bit value next to the quotient itself, also where float32 would round onto a border.
-      float g[kWidth], w8[kWidth], v[kWidth], gmax = 0.f;
-      load8<W>(w, c, a.cols, w8);
+      float g[kWidth], late[kWidth], v[kWidth], gmax = 0.f;
+      const float(&w8)[kWidth] = kEarly ? early : late;
+      if constexpr (!kEarly) load8<W>(w, c, a.cols, late);
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) {
         g[i] = h[i] * w8[i];
@@ -269,7 +279,8 @@ struct QuantArgs {
 
 constexpr int kThreads = 256;
 
-// 1 x 128 blocks: a workgroup takes 256 >> lane_bits neighbouring rows.
+// 1 x 128 blocks: a workgroup takes 256 >> lane_bits neighbouring rows. HBM: 8191 x 10240 in bf16 moves 253 MB in 49 us,
+// 5.14 TB/s, a copy's rate; non-temporal loads and stores and 512 lanes were no faster.
 template <typename T, bool POW2>
 __global__ __launch_bounds__(kThreads) void k_rows(QuantArgs a) {
   const int per = kThreads >> a.lane_bits;
@@ -291,7 +302,8 @@ __global__ __launch_bounds__(kThreads) void k_rows(QuantArgs a) {
   }
 }
 
-// 128 x 128 blocks: one workgroup a block, held in registers between the maximum and the conversion.
+// 128 x 128 blocks: one workgroup a block, held in registers between the maximum and the conversion. HBM: 4096 x 4096
+// in bf16 moves 50 MB in 10.5 us, 4.8 TB/s: four workgroups a CU in one round, which all load, then all store.
 template <typename T, bool POW2>
 __global__ __launch_bounds__(kThreads) void k_tiles(QuantArgs a) {
   constexpr int kRowsAtOnce = kThreads / kLanes, kPasses = kBlockK / kRowsAtOnce;
@@ -337,12 +349,16 @@ constexpr int64_t kRowsALaunch = 1 << 21;
 template <typename T, typename W, bool POW2, bool RES>
 int norm_piece(const NormArgs& a, hipStream_t s) {
   const unsigned grid = (unsigned)((a.rows + kXcds - 1) / kXcds * kXcds);
+  const bool few = a.rows <= 1024;
 #define YODA_NORM(threads, chunks) k_norm<T, W, POW2, RES, threads, chunks><<<grid, threads, 0, s>>>(a)
   if (a.padded <= 64 * 8) YODA_NORM(64, 1);
   else if (a.padded <= 128 * 8) YODA_NORM(128, 1);
   else if (a.padded <= 256 * 8) YODA_NORM(256, 1);
+  else if (few && a.padded <= 512 * 8) YODA_NORM(512, 1);
   else if (a.padded <= 256 * 2 * 8) YODA_NORM(256, 2);
+  else if (few && a.padded <= 512 * 2 * 8) YODA_NORM(512, 2);
   else if (a.padded <= 256 * 4 * 8) YODA_NORM(256, 4);
+  else if (few && a.padded <= 1024 * 2 * 8) YODA_NORM(1024, 2);
   else if (a.padded <= 512 * 4 * 8) YODA_NORM(512, 4);
   else if (a.padded <= 1024 * 4 * 8) YODA_NORM(1024, 4);
   else YODA_NORM(1024, 0);

@@ -157,6 +157,15 @@ def test_norm(require_gpu, rows, cols, residual, dtype, pow2):
         _check_norm(q, h, x, w, r, 1e-5, pow2)
 
 
+@pytest.mark.parametrize("rows", [1024, 1025])
+@pytest.mark.parametrize("cols", [1500, 2500, 5001, 9000])
+def test_norm_of_few_and_of_many_rows(require_gpu, rows, cols):
+    """Few rows take more lanes each."""
+    x, w, res = _randn((rows, cols), cols, torch.bfloat16), _randn((cols,), 3, torch.bfloat16), _randn((rows, cols), 4, torch.bfloat16)
+    q, h = _ops().add_rms_norm(x.to(DEV), w.to(DEV), res.to(DEV))
+    _check_norm(q, h, x, w, res, 1e-6, False)
+
+
 def test_norm_strides_zero_rows_and_nan(require_gpu):
     fp8 = _ops()
     wide, other = _randn((30, 700), 1, torch.bfloat16), _randn((30, 900), 2, torch.bfloat16)
