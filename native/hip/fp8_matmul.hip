@@ -108,7 +108,9 @@ __device__ __forceinline__ bool tile_of(int block, int tiles_m, int tiles_n, int
   return true;
 }
 
-// A lane's MT rows from m on; n: the wave's first column.
+// A lane's MT rows from m on; n: the wave's first column. Four pieces at a time, so that the two stores to a line of
+// 128 bytes follow each other and reach memory as one (two pieces at a time wrote 49 MB instead of 34 for 4096 x 4096 x
+// 4096 and took 62.1 us instead of 61.2; 8192 x 8192 x 8192 399 : 393).
 template <int MT, int NT, typename O>
 __device__ __forceinline__ void store_tile(const MatArgs& p, const f32x4 (&acc)[MT][NT], int64_t m, int64_t n, int g) {
   using B = typename Bits<O>::type;
@@ -116,34 +118,33 @@ __device__ __forceinline__ void store_tile(const MatArgs& p, const f32x4 (&acc)[
   if (m >= p.m) return;
   const int rows = (int)min((int64_t)MT, p.m - m);
 #pragma unroll
-  for (int j = 0; j < NT; j += 2) {
-    const int64_t at = n + 16 * j;
+  for (int four = 0; four < NT; four += 4) {
+    const int64_t at = n + 16 * four;
     if (at >= p.n) break;
-    float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float bias[16] = {};
     if (p.bias) {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) bias[r] = load_f32<O>(((const B*)p.bias)[min(at + r, p.n - 1)]);
+      for (int r = 0; r < 16; ++r) bias[r] = load_f32<O>(((const B*)p.bias)[min(at + (r & 7) + 4 * (r & 8), p.n - 1)]);
     }
     B* out = (B*)p.out + m * p.pitch + at;
-    if (at + 8 <= p.n) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        if (i >= rows) break;
-        const f32x4 u = acc[i][j], v = acc[i][j + 1];
-        Wide<sizeof(B)>::store(out, u32x4{pack2<O>(u[0] + bias[0], u[1] + bias[1]), pack2<O>(u[2] + bias[2], u[3] + bias[3]),
-                                          pack2<O>(v[0] + bias[4], v[1] + bias[5]), pack2<O>(v[2] + bias[6], v[3] + bias[7])});
-        out += p.pitch;
+    for (int i = 0; i < MT; ++i) {
+      if (i >= rows) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 u = acc[i][four + 2 * h], v = acc[i][four + 2 * h + 1];
+        const float* add = bias + 8 * h;
+        const int64_t left = p.n - at - 32 * h;
+        if (left >= 8) {
+          Wide<sizeof(B)>::store(out + 32 * h, u32x4{pack2<O>(u[0] + add[0], u[1] + add[1]), pack2<O>(u[2] + add[2], u[3] + add[3]),
+                                                     pack2<O>(v[0] + add[4], v[1] + add[5]), pack2<O>(v[2] + add[6], v[3] + add[7])});
+        } else {
+#pragma unroll
+          for (int r = 0; r < 7; ++r)
+            if (r < left) out[32 * h + r] = store_bits<O>((r < 4 ? u[r & 3] : v[r & 3]) + add[r]);
+        }
       }
-    } else {
-      const int cols = (int)(p.n - at);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        if (i >= rows) break;
-#pragma unroll
-        for (int r = 0; r < 7; ++r)
-          if (r < cols) out[r] = store_bits<O>((r < 4 ? acc[i][j][r & 3] : acc[i][j + 1][r & 3]) + bias[r]);
-        out += p.pitch;
-      }
+      out += p.pitch;
     }
   }
 }
@@ -164,6 +165,12 @@ __device__ __forceinline__ void store_tile(const MatArgs& p, const f32x4 (&acc)[
 // and waits for those that the quarter reads, and the barrier joins the waits of all four. What a
 // quarter loads into was read a step before (x0: waited for by count at Q0; the others: their
 // products have been issued).
+//
+// 8192 x 8192 x 8192: 393 to 398 us, 2.8 PFLOP/s (a library's product with one scale for each matrix: 355 us), 4096 x 4096 x
+// 4096: 53 us. The matrix units are busy 72 % of the time at 1.93 GHz, to which the card's power holds the
+// clock (at 84 % the library runs at 1.76). Per step the reads and loads take as long in LDS as the products: with no
+// loads 358 us, with no reads 346, with neither 306. Two meetings a step, 2, 8 or 16 rows of tiles a column and
+// non-temporal stores were no faster. The stores of a round of tiles are 5 us of the 100, at the memory's rate.
 struct Quarters {
   static constexpr int BM = 256, BN = 256;
   static constexpr int kPart = 128 * kBlockK;                     // x0, x1, w0 or w1 of one step: 16 KB
@@ -333,6 +340,11 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
 //   after the first meeting   w(k+2) and rows' pieces 0-3 (k+2)    (read in step k-1)
 //   after the second          rows' pieces 4-7 (k+2), rows' scales (k+3)
 // so a load has a step and a half to arrive. Each wave counts its own loads: 6 and 3.
+//
+// 4096 x 4096 x 4096: 59 to 61 us, 2.3 PFLOP/s, the matrix units busy 64 % of the time; 4096 x 10240 x 4096: 167 us
+// for two and a half rounds of tiles. Bound as k_quarters is, with 192 KB a step read from LDS instead of
+// 128: e8m0 scales take 53 us. (Four waves of 128 x 128 would hold 256 sums a lane, which leaves
+// no vector registers for the multiply-adds.)
 struct Eight {
   static constexpr int BM = 256, BN = 256;
   static constexpr int kRows = 128 * kBlockK;                     // half of the rows' pieces: 16 KB
@@ -516,6 +528,12 @@ __device__ __forceinline__ void store4(const MatArgs& p, f32x4 v, int64_t m, int
 // reads all rows again (out of L2, 33 TB/s) and a piece of the weight (out of HBM) that nobody else reads.
 // K is in gridDim.y parts, whose float32 sums go to a workspace and are joined by k_join in the order of the parts. Where two
 // workgroups' stages fit in LDS, they share a CU and one runs while the other waits.
+//
+// 128 x 128: 0.44 us a step where the products take 0.21: 64 KB of reads and 32 KB of loads go through LDS.
+// 777 x 5000 x 1928 takes 17 us, 0.88 PFLOP/s (280 tiles, so some CUs have two); 4096 x 2048 x 4096 34, 2.05 PFLOP/s.
+// 256 x 128 by eight waves of 64 x 64 was no faster (17.5 and 34), by four of 128 x 64 slower (22 and 39).
+// 128 x 32: 128 x 8192 x 4096 takes 14 us with float scales, 12 with e8m0, 2.6 TB/s: 256 workgroups, each of which
+// starts, runs 32 steps of 0.26 us as its 20 KB a step arrive, and stores.
 template <int RP_, int CP_>
 struct Mid {
   static constexpr int RP = RP_, CP = CP_, BM = 32 * RP, BN = 32 * CP;
@@ -692,7 +710,8 @@ __global__ __launch_bounds__(256, 2) void k_mid(MatArgs p, int tiles_m, int tile
   }
 }
 
-// out = the sum of the parts in their order, plus bias: four neighbours a lane, a tile every RP * CP workgroups.
+// out = the sum of the parts in their order, plus bias: four neighbours a lane, a tile every RP * CP workgroups. The parts
+// come out of the caches; what it costs is a launch, about 2.5 us with the parts' stores.
 template <int RP, int CP, typename O>
 __global__ __launch_bounds__(256) void k_join(MatArgs p, int tiles_m, int tiles_n, const f32x4* parts, int count) {
   const int tile = blockIdx.x / (RP * CP), at = blockIdx.x % (RP * CP) * 256 + threadIdx.x;
@@ -727,6 +746,8 @@ int run_mid(const MatArgs& p, bool pow2, int count, float* parts, hipStream_t s)
 // blocks ahead, each weight byte once on the whole card; the rows are read again by each workgroup, out of L2.
 // No wave waits for another until the end, when the waves' sums are added through LDS in the order of
 // the waves. Lane (c, g) has row c; columns as in column_of where NP is 2.
+// 16 x 8192 x 8192 takes 13.6 us, 5.0 TB/s of the 6.1 that reads reach; 1 x 4096 x 4096 5.2, of which 2.8 are the
+// bytes at that rate and the rest a launch. Tiles through LDS take 14.9 for the former.
 template <int NP, int WAVES, int DEPTH, typename O, bool POW2>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_narrow(MatArgs p) {
   __shared__ f32x4 part[WAVES * NP * 64];
@@ -841,8 +862,8 @@ int narrow(const MatArgs& p, bool pow2, hipStream_t s) {
 //   256 x 256       (10.5 + 1.4 a step, float scales 1.57) a round of 256; a last round of a share f counts (1 + f) / 2
 // Measured, this one : the next best, e8m0 scales: 16 x 8192 x 8192 few rows 13.4 : 14.9 32 x 32;
 // 32 x 8192 x 8192 32 x 32 14.7 : 16.1 64 x 32; 64 x 8192 x 8192 64 x 32 15.3 : 16.7 64 x 64; 128 x 8192 x 4096 128 x 32
-// 11.9 : 15.2 128 x 128 in two parts; 2048 x 2048 x 4096 128 x 128 23 : 44 256 x 256; 4096 x 4096 x 4096 256 x 256
-// 55 : 64 128 x 128.
+// 12 : 15 128 x 128 in two parts; 2048 x 2048 x 4096 128 x 128 23 : 44 256 x 256; 4096 x 4096 x 4096 256 x 256
+// 53 : 64 128 x 128.
 struct Shape {
   int rows, columns;                    // pieces of 32
   double one, two, round;               // us a step alone on a CU, of two on a CU; and a round's own
