@@ -463,6 +463,24 @@ def test_interpod_affinity_native_equals_python_on_random_clusters(case):
     assert native_scores(eng, p, feas) == {x.name: x.score for x in out}
 
 
+def test_a_namespace_that_a_term_names_twice_counts_once():
+    """Nine pods on n0, one on n1; one of the nine prefers the new pod's node, which counts against the
+    new pod's own preference in the normalized scores."""
+    nodes = [{"metadata": {"name": f"n{i}", "labels": {HOST: f"n{i}"}},
+              "status": {"allocatable": {"cpu": "64", "memory": "512Gi", "pods": "110"}}} for i in range(3)]
+    term = {"topologyKey": HOST, "labelSelector": {}}
+    likes = {"podAffinity": {"preferredDuringSchedulingIgnoredDuringExecution": [{"weight": 1, "podAffinityTerm": term}]}}
+    placed = [{"metadata": {"name": f"q{j}", "namespace": "default", "uid": f"q{j}-{next(_uid)}", "labels": {}},
+               "spec": {"nodeName": "n1" if j == 9 else "n0", **({"affinity": likes} if j == 8 else {})}}
+              for j in range(10)]
+    for names in (["default", "default"], ["default", "ml", "default"], ["ml", "ml"]):
+        for selector in ({}, {"matchLabels": {"app": "a"}}):
+            avoids = {"weight": 1, "podAffinityTerm": {"topologyKey": HOST, "labelSelector": selector, "namespaces": names}}
+            newp = {"metadata": {"name": "new", "namespace": "default", "uid": f"new-{next(_uid)}", "labels": {}},
+                    "spec": {"affinity": {"podAntiAffinity": {"preferredDuringSchedulingIgnoredDuringExecution": [avoids]}}}}
+            test_interpod_affinity_native_equals_python_on_random_clusters.hypothesis.inner_test((nodes, placed, newp, 0))
+
+
 def test_affinity_term_sets_follow_release_and_node_removal():
     """The engine groups reserved pods' (anti-)affinity terms by term set with per-node holder
     counts. After releases and a node removal, its filter verdicts and scores equal those of an
