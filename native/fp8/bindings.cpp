@@ -6,6 +6,8 @@
 // as a number. The C entries of libyoda_hip.so are bound by address, so this module links to torch alone.
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/hip/EmptyTensor.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -46,17 +48,22 @@ bool neighbours(const at::Tensor& t, int64_t n, const at::Device& device) {
          !t.is_neg() && !recorded(t);
 }
 
+// a new tensor next to x, straight from the device's allocator (the dispatcher's way to it takes longer)
+at::Tensor room(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& x) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, x.device(), std::nullopt));
+}
+
 at::Tensor values_for(const at::Tensor& x) {
-  return at::empty({x.size(0), (x.size(1) + kBlock - 1) / kBlock * kBlock}, x.options().dtype(at::kFloat8_e4m3fn));
+  return room({x.size(0), (x.size(1) + kBlock - 1) / kBlock * kBlock}, at::kFloat8_e4m3fn, x);
 }
 
 // the scales' layout: 1 x 128 blocks [blocks of K][rows to a multiple of 8], as [rows, blocks]; 128 x 128 [rows' blocks][blocks of K to one of 4]
 at::Tensor scales_for(const at::Tensor& x, bool tiles, bool pow2) {
-  const auto options = x.options().dtype(pow2 ? at::kFloat8_e8m0fnu : at::kFloat);
+  const auto type = pow2 ? at::kFloat8_e8m0fnu : at::kFloat;
   const int64_t kb = (x.size(1) + kBlock - 1) / kBlock;
-  if (tiles) return at::empty({(x.size(0) + kBlock - 1) / kBlock, (kb + 3) / 4 * 4}, options);
+  if (tiles) return room({(x.size(0) + kBlock - 1) / kBlock, (kb + 3) / 4 * 4}, type, x);
   const int64_t pitch = (x.size(0) + 7) / 8 * 8;
-  return at::empty_strided({pitch, kb}, {1, pitch}, options);
+  return at::Tensor(at::detail::empty_strided_cuda({pitch, kb}, {1, pitch}, type, x.device()));
 }
 
 // whether values and scales are those of a block matrix of these sizes
@@ -71,12 +78,15 @@ bool laid_out(const at::Tensor& v, const at::Tensor& s, const at::Device& device
   return s.size(0) == pitch && s.size(1) == kb && (pitch == 0 || kb == 1 || s.stride(1) == pitch) && (pitch <= 1 || s.stride(0) == 1);
 }
 
+// the current stream of a tensor's device
+void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
 PyObject* refused() { Py_RETURN_NONE; }
 
-// norm(x, weight, residual or None, eps, pow2, stream) -> (values, scales, stream or None)
+// norm(x, weight, residual or None, eps, pow2) -> (values, scales, sum or None)
 PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
-  if (count != 6) return refused();
+  if (count != 5) return refused();
   const at::Tensor *x = tensor(args[0]), *w = tensor(args[1]), *r = tensor(args[2]);
   if (!x || !w || (!r && args[2] != Py_None) || !matrix(*x)) return refused();
   const int64_t rows = x->size(0), cols = x->size(1);
@@ -87,16 +97,15 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return refused();
   const double eps = PyFloat_AsDouble(args[3]);
   const long pow2 = PyLong_AsLong(args[4]);
-  void* stream = PyLong_AsVoidPtr(args[5]);
   if (PyErr_Occurred()) return nullptr;
   if (!(eps >= 0) || cols > (1 << 30)) return refused();
   at::Tensor q = values_for(*x), s = scales_for(*x, false, pow2), h;
-  if (r) h = at::empty({rows, cols}, x->options());
+  if (r) h = room({rows, cols}, x->scalar_type(), *x);
   // (what may throw comes before the lock is given up)
   const int device = x->get_device(), type = type_of(x->scalar_type());
   const int64_t pitch = x->stride(0), r_pitch = r ? r->stride(0) : 0;
   const void *from = x->data_ptr(), *add = r ? r->data_ptr() : nullptr, *by = w->data_ptr();
-  void *sum = r ? h.data_ptr() : nullptr, *values = q.data_ptr(), *scales = s.data_ptr();
+  void *stream = stream_of(*x), *sum = r ? h.data_ptr() : nullptr, *values = q.data_ptr(), *scales = s.data_ptr();
   int rc = 0;
   Py_BEGIN_ALLOW_THREADS
   rc = norm_entry(device, stream, type, wide, pow2 != 0, from, pitch, add, r_pitch, by, sum, values, scales, rows, (int)cols, eps);
@@ -116,19 +125,18 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
-// quantize(x, tiles, pow2, stream) -> (values, scales)
+// quantize(x, tiles, pow2) -> (values, scales)
 PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
-  const at::Tensor* x = count == 4 ? tensor(args[0]) : nullptr;
+  const at::Tensor* x = count == 3 ? tensor(args[0]) : nullptr;
   if (!x || !matrix(*x) || x->size(1) > (1 << 30)) return refused();
   const long tiles = PyLong_AsLong(args[1]), pow2 = PyLong_AsLong(args[2]);
-  void* stream = PyLong_AsVoidPtr(args[3]);
   if (PyErr_Occurred()) return nullptr;
   at::Tensor q = values_for(*x), s = scales_for(*x, tiles, pow2);
   const int device = x->get_device(), type = type_of(x->scalar_type());
   const int64_t pitch = x->stride(0), rows = x->size(0), cols = x->size(1);
   const void* from = x->data_ptr();
-  void *values = q.data_ptr(), *scales = s.data_ptr();
+  void *stream = stream_of(*x), *values = q.data_ptr(), *scales = s.data_ptr();
   int rc = 0;
   Py_BEGIN_ALLOW_THREADS
   rc = quantize_entry(device, stream, type, tiles != 0, pow2 != 0, from, pitch, values, scales, rows, (int)cols);
@@ -142,17 +150,16 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
-// matmul(a's values, a's scales, b's values, b's scales, rows, columns, K, type of out, bias or None, out or None, stream) -> out
+// matmul(a's values, a's scales, b's values, b's scales, rows, columns, K, type of out, bias or None, out or None) -> out
 // (values and scales are a BlockMatrix's own, laid out by it)
 PyObject* matmul(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
-  if (count != 11) return refused();
+  if (count != 10) return refused();
   const at::Tensor *a = tensor(args[0]), *sa = tensor(args[1]), *b = tensor(args[2]), *sb = tensor(args[3]),
                    *bias = tensor(args[8]), *given = tensor(args[9]);
   if (!a || !sa || !b || !sb || (!bias && args[8] != Py_None) || (!given && args[9] != Py_None)) return refused();
   const int64_t m = PyLong_AsLongLong(args[4]), n = PyLong_AsLongLong(args[5]), k = PyLong_AsLongLong(args[6]);
   const long type = PyLong_AsLong(args[7]);
-  void* stream = PyLong_AsVoidPtr(args[10]);
   if (PyErr_Occurred()) return nullptr;
   const at::Device device = a->device();
   const at::ScalarType out_type = type == 0 ? at::kBFloat16 : at::kHalf;
@@ -169,22 +176,39 @@ PyObject* matmul(PyObject*, PyObject* const* args, Py_ssize_t count) {
       return refused();
     if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();        // written in place
   } else {
-    out = at::empty({m, n}, a->options().dtype(out_type));
+    out = room({m, n}, out_type, *a);
   }
   const int pow2 = sa->scalar_type() != at::kFloat;
   const int64_t bytes = workspace_entry(m, n, kb, pow2);
-  at::Tensor room;
-  if (bytes) room = at::empty({bytes}, a->options().dtype(at::kByte));
+  at::Tensor workspace;
+  if (bytes) workspace = room({bytes}, at::kByte, *a);
   const int64_t pitch = m > 1 ? out.stride(0) : std::max<int64_t>(n, 1);
   const void *pa = a->data_ptr(), *psa = sa->data_ptr(), *pb = b->data_ptr(), *psb = sb->data_ptr(),
              *add = bias ? bias->data_ptr() : nullptr;
-  void *to = out.data_ptr(), *space = bytes ? room.data_ptr() : nullptr;
+  void *stream = stream_of(*a), *to = out.data_ptr(), *space = bytes ? workspace.data_ptr() : nullptr;
   int rc = 0;
   Py_BEGIN_ALLOW_THREADS
   rc = matmul_entry(device.index(), stream, (int)type, pow2, pa, psa, pb, psb, add, to, m, n, kb, pitch, (m + 7) / 8 * 8, space, bytes);
   Py_END_ALLOW_THREADS
   if (rc) return PyLong_FromLong(rc);
   return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// corner(t, rows, columns) -> a view of t's first rows and columns, or None where torch has to make it (of a tensor
+// that is part of a graph). A slice in Python takes 2 us, and every call's result is asked for its values and scales.
+PyObject* corner(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* t = count == 3 ? tensor(args[0]) : nullptr;
+  if (!t || !t->is_cuda() || t->layout() != at::kStrided || t->dim() != 2 || t->requires_grad() || t->is_inference() || t->is_neg())
+    return refused();
+  const int64_t rows = PyLong_AsLongLong(args[1]), cols = PyLong_AsLongLong(args[2]);
+  if (PyErr_Occurred()) return nullptr;
+  if (rows < 0 || cols < 0 || rows > t->size(0) || cols > t->size(1)) return refused();
+  const c10::TensorImpl* from = t->unsafeGetTensorImpl();
+  at::Tensor view(from->shallow_copy_and_detach(from->version_counter(), /*allow_tensor_metadata_change=*/true));
+  view.unsafeGetTensorImpl()->set_sizes_and_strides({rows, cols}, t->strides(), t->storage_offset());
+  return THPVariable_Wrap(std::move(view));
   END_HANDLE_TH_ERRORS
 }
 
@@ -207,6 +231,7 @@ PyMethodDef methods[] = {
     {"norm", (PyCFunction)(void (*)())norm, METH_FASTCALL, nullptr},
     {"quantize", (PyCFunction)(void (*)())quantize, METH_FASTCALL, nullptr},
     {"matmul", (PyCFunction)(void (*)())matmul, METH_FASTCALL, nullptr},
+    {"corner", (PyCFunction)(void (*)())corner, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

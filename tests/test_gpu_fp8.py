@@ -547,6 +547,26 @@ def test_more_columns_than_a_launch_takes(require_gpu, m):
         assert ((got - want).abs() <= mass * (7 * 2.0 ** -13 + 256 * 2.0 ** -24) + want.abs() * 2.0 ** -8).all()
 
 
+def test_values_and_scales_are_views(require_gpu):
+    fp8 = _ops()
+    x = _randn((5, 200), 8).to(DEV)
+    for m in (fp8.quantize(x), fp8.quantize(x, 128), fp8.quantize(x, 1, E8M0)):
+        for view, whole, like in ((m.values, m.data, m.data[:5, :200]), (m.scales, m._room, m._room[:m.scales.shape[0], :2])):
+            assert view.shape == like.shape and view.stride() == like.stride() and view.data_ptr() == whole.data_ptr()
+            assert view.dtype == whole.dtype and not view.requires_grad
+            assert torch.equal(view.float(), like.float())
+    m = fp8.quantize(x)
+    scales, before = m.scales, m._room._version
+    m._room.mul_(2)                                            # what is written to the whole is seen in its views
+    assert torch.equal(scales, m._room[:5]) and scales._version == m._room._version > before
+    with torch.inference_mode():
+        inner = fp8.quantize(x)
+        assert torch.equal(inner.scales, fp8.quantize(x).scales) and inner.values.shape == (5, 200)
+    learned = fp8.BlockMatrix(m.values, m.scales.clone().requires_grad_())
+    (grad,) = torch.autograd.grad(learned.scales.sum(), learned._room)
+    assert torch.equal(grad[:5], torch.ones_like(grad[:5])) and not grad[5:].any()
+
+
 def test_out_counts_as_written(require_gpu):
     fp8 = _ops()
     a, b = fp8.quantize(torch.ones(4, 128, device=DEV)), fp8.quantize(torch.ones(8, 128, device=DEV), 128)

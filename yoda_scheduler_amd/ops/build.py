@@ -72,7 +72,7 @@ ARTEFACTS: dict[str, dict] = {
                              "common/build_id.h"],
                     "recipe": "g++ -O2 -std=c++17 -lamd_smi v2"},
     "fp8": {"out": f"_yoda_fp8{EXT}", "srcs": ["fp8/bindings.cpp"], "deps": ["fp8/bindings.cpp", "common/build_id.h"],
-            "recipe": "g++ -O2 -std=c++17 -fPIC -shared -fvisibility=hidden -ltorch_python v1"},
+            "recipe": "g++ -O2 -std=c++17 -fPIC -shared -fvisibility=hidden -ltorch_hip -ltorch_python v2"},
     "hip": {"out": "libyoda_hip.so", "srcs": None, "deps": None,     # every native/hip/*.hip + *.h
             "recipe": f"hipcc --offload-arch={ARCH} -O3 -std=c++17 -fPIC -shared -packed-fp32-ops v3"},
 }
@@ -237,16 +237,17 @@ def torch_root() -> Path | None:
 def build_fp8(force: bool = False) -> list[Path]:
     """The 8-bit operators' torch module; nothing where torch or its headers are missing (the scheduler's image)."""
     torch = torch_root()
-    if torch is None or not (torch / "include" / "ATen" / "ATen.h").exists():
+    if torch is None or not all((torch / p).exists() for p in ("include/ATen/hip/EmptyTensor.h", "lib/libtorch_hip.so")):
         return []
     out = out_path("fp8")
     if force or _stale("fp8"):
         bid = source_hash("fp8")
         inc = [f"-I{torch / 'include'}", f"-I{torch / 'include/torch/csrc/api/include'}",
-               f"-I{sysconfig.get_paths()['include']}", f"-I{NATIVE / 'common'}"]
+               f"-I{sysconfig.get_paths()['include']}", f"-I{NATIVE / 'common'}", f"-I{ROCM / 'include'}",
+               "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"]
         _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
               "-Wno-unused-function", "-D_GLIBCXX_USE_CXX11_ABI=1", _bid_flag(bid), *inc, *_srcs("fp8"), "-o", str(out),
-              f"-L{torch / 'lib'}", f"-Wl,-rpath,{torch / 'lib'}", "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python"],
+              f"-L{torch / 'lib'}", f"-Wl,-rpath,{torch / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python"],
              "8-bit operators' torch module")
         _record("fp8", bid)
     return [out]

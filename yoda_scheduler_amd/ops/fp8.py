@@ -54,6 +54,12 @@ def blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
+def _corner(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """A view of the first rows and columns."""
+    view = _module.corner(t, rows, cols) if _module is not None else None
+    return t[:rows, :cols] if view is None else view
+
+
 def _scales(like: torch.Tensor, rows: int, kb: int, block_rows: int, dtype: torch.dtype) -> torch.Tensor:
     """Room for the scales of ``rows`` (of blocks) x ``kb`` blocks and their padding, in the kernels' layout."""
     if block_rows == 1:
@@ -120,16 +126,16 @@ class BlockMatrix:
     @property
     def values(self) -> torch.Tensor:
         """[rows, cols] e4m3: a view without the padding."""
-        return self.data if self.cols % BLOCK == 0 else self.data[:, :self.cols]
+        return self.data if self.cols % BLOCK == 0 else _corner(self.data, self.rows, self.cols)
 
     @property
     def scales(self) -> torch.Tensor:
         """[blocks of rows, blocks of columns]: a view without the padding."""
         r, kb = self._room.shape
         if self.block_rows == 1:
-            return self._room if r == self.rows else self._room[:self.rows]
+            return self._room if r == self.rows else _corner(self._room, self.rows, kb)
         want = self.data.shape[1] // BLOCK
-        return self._room if kb == want else self._room[:, :want]
+        return self._room if kb == want else _corner(self._room, r, want)
 
     @property
     def shape(self) -> tuple[int, int]:
@@ -142,13 +148,6 @@ class BlockMatrix:
     def __repr__(self) -> str:
         return (f"BlockMatrix({self.rows}x{self.cols}, blocks {self.block_rows}x{BLOCK}, "
                 f"scales {self._room.dtype}, {self.data.device})")
-
-
-_current_stream = torch._C._cuda_getCurrentRawStream    # torch.cuda.current_stream makes an object first: 2 us
-
-
-def _stream_of(x: torch.Tensor) -> int:
-    return _current_stream(x.get_device()) if isinstance(x, torch.Tensor) and x.is_cuda else 0
 
 
 def _refuse_matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None) -> None:
@@ -197,7 +196,7 @@ def quantize(x: torch.Tensor, block_rows: int = 1, scale_dtype: torch.dtype = to
     if block_rows not in (1, BLOCK):
         raise ValueError(f"block_rows: 1 or {BLOCK}, not {block_rows}")
     pow2 = _scale_kind(scale_dtype)
-    got = _native().quantize(x, block_rows == BLOCK, pow2, _stream_of(x))
+    got = _native().quantize(x, block_rows == BLOCK, pow2)
     if type(got) is tuple:
         rows, cols = x.shape
         return BlockMatrix._of(*got, rows, cols, block_rows)
@@ -218,7 +217,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     one of zeros where eps is 0.
     """
     pow2 = _scale_kind(scale_dtype)
-    got = _native().norm(x, weight, residual, eps, pow2, _stream_of(x))
+    got = _native().norm(x, weight, residual, eps, pow2)
     if type(got) is tuple:
         rows, cols = x.shape
         return BlockMatrix._of(got[0], got[1], rows, cols, 1), got[2]
@@ -258,7 +257,7 @@ def matmul(a: BlockMatrix, b: BlockMatrix, out_dtype: torch.dtype = torch.bfloat
     """
     kind = _OUT.get(out_dtype)
     if kind is not None and a.block_rows == 1 and b.block_rows == BLOCK and a.cols == b.cols:
-        got = _native().matmul(a.data, a._room, b.data, b._room, a.rows, b.rows, a.cols, kind, bias, out, _stream_of(a.data))
+        got = _native().matmul(a.data, a._room, b.data, b._room, a.rows, b.rows, a.cols, kind, bias, out)
         if isinstance(got, torch.Tensor):
             return out if out is not None else got
         if got:
