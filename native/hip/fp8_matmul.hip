@@ -341,8 +341,8 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
 //   after the second          rows' pieces 4-7 (k+2), rows' scales (k+3)
 // so a load has a step and a half to arrive. Each wave counts its own loads: 6 and 3.
 //
-// 4096 x 4096 x 4096: 59 to 61 us, 2.3 PFLOP/s, the matrix units busy 64 % of the time; 4096 x 10240 x 4096: 167 us
-// for two and a half rounds of tiles. Bound as k_quarters is, with 192 KB a step read from LDS instead of
+// 4096 x 4096 x 4096: 59 to 61 us, 2.3 PFLOP/s, the matrix units busy 64 % of the time; 8192 x 8192 x 8192: 446 to 450.
+// Bound as k_quarters is, with 192 KB a step read from LDS instead of
 // 128: e8m0 scales take 53 us. (Four waves of 128 x 128 would hold 256 sums a lane, which leaves
 // no vector registers for the multiply-adds.)
 struct Eight {
@@ -880,17 +880,21 @@ struct Plan {
   enum { kNarrow, kSmall, k256 } kind;
   int shape, parts;
   int64_t groups, bytes;                // workgroups; bytes of workspace
+  double us;
+  int64_t split;                        // columns from 0 on that tiles of 256 x 256 take before
 };
 
-Plan plan(int64_t m, int64_t n, int kb, bool pow2) {
+double round_of_256(int kb, bool pow2) { return 10.5 + kb * (pow2 ? 1.4 : 1.57); }
+
+Plan one_kind(int64_t m, int64_t n, int kb, bool pow2) {
   const double weight = (double)n * kb * kBlockK;
-  Plan best = {Plan::k256, 0, 1, 0, 0};
+  Plan best = {Plan::k256, 0, 1, 0, 0, 0, 0};
   const int64_t big = (m + 255) / 256 * ((n + 255) / 256);
   const double rest = big % 256 ? (1 + big % 256 / 256.0) / 2 : 0;
-  double least = std::max<double>(big / 256 + rest, 1) * (10.5 + kb * (pow2 ? 1.4 : 1.57));
+  double least = std::max<double>(big / 256 + rest, 1) * round_of_256(kb, pow2);
   if (m <= 16 && n < kMostGroups * 32) {
     const double t = 2 + weight * 1.5 / 8e6 + 3. * ((n + 8191) / 8192 - 1);
-    if (t < least) least = t, best = {Plan::kNarrow, 0, 1, 0, 0};
+    if (t < least) least = t, best = {Plan::kNarrow, 0, 1, 0, 0, 0, 0};
   }
   for (int shape = 0; shape < 4; ++shape) {
     const Shape& h = kShapes[shape];
@@ -903,16 +907,39 @@ Plan plan(int64_t m, int64_t n, int kb, bool pow2) {
       double t = groups <= 256 ? 5 + steps * (pow2 ? h.one : h.one_f) : 2 + rounds * (h.round + steps * (pow2 ? h.two : h.two_f));
       t = std::max(t, 3 + weight / 5.3e6);
       if (parts > 1) t += 2.5 + 2 * bytes / 5e6;
-      if (t < least) least = t, best = {Plan::kSmall, shape, parts, groups, bytes};
+      if (t < least) least = t, best = {Plan::kSmall, shape, parts, groups, bytes, 0, 0};
     }
   }
+  best.us = least;
   return best;
 }
 
+Plan plan(int64_t m, int64_t n, int kb, bool pow2) {
+  Plan best = one_kind(m, n, kb, pow2);
+  // Tiles of 256 x 256 for as many whole rounds as there are, and what else suits the columns that are left: 4608 x 4096 x
+  // 4096 takes 73 us instead of 93, 4096 x 4100 x 900 29 instead of 38, 4096 x 10240 x 4096 148 instead of 153.
+  const int64_t tm = (m + 255) / 256, tn = (n + 255) / 256, most = tm * tn / 256 * 256 / tm;
+  if (most < 1 || most >= tn) return best;
+  Plan rest = one_kind(m, n - 256 * most, kb, pow2);
+  rest.us += 2 + (double)((tm * most + 255) / 256) * round_of_256(kb, pow2);
+  rest.split = 256 * most;
+  return rest.kind != Plan::k256 && rest.us < best.us ? rest : best;
+}
+
 template <typename O>
-int run(const MatArgs& p, bool pow2, float* workspace, int64_t bytes, hipStream_t s) {
+int run(MatArgs p, bool pow2, float* workspace, int64_t bytes, hipStream_t s) {
   const Plan to = plan(p.m, p.n, p.kb, pow2);
   if (to.bytes > bytes || (to.bytes && !workspace)) return -1;
+  if (to.split) {
+    MatArgs first = p;
+    first.n = to.split;
+    if (const int rc = run_256<O>(first, pow2, s)) return rc;
+    p.n -= to.split;
+    p.b += to.split * p.kb * kBlockK;
+    p.sb = (const uint8_t*)p.sb + to.split / kBlockK * p.sb_pitch * (pow2 ? 1 : 4);
+    p.out = (uint16_t*)p.out + to.split;
+    if (p.bias) p.bias = (const uint16_t*)p.bias + to.split;
+  }
   if (to.kind == Plan::k256) return run_256<O>(p, pow2, s);
   // two pieces of columns a workgroup halve what is read of the rows, where that leaves enough workgroups
   if (to.kind == Plan::kNarrow) return p.n >= 8192 ? narrow<2, 8, 4, O>(p, pow2, s) : narrow<1, 8, 4, O>(p, pow2, s);

@@ -286,7 +286,10 @@ def test_matmul_large(require_gpu, k, pow2):
                                         (31, 9000, 1500, False), (64, 512, 16_384, True), (64, 512, 16_384, False),
                                         (50, 9000, 900, True), (100, 200, 12_000, True), (100, 200, 12_000, False),
                                         (128, 9000, 640, False), (130, 130, 9000, True), (500, 900, 5000, False),
-                                        (512, 8192, 1000, True), (777, 5000, 500, False), (1024, 2000, 700, True)])
+                                        (512, 8192, 1000, True), (777, 5000, 500, False), (1024, 2000, 700, True),
+                                        # whole rounds of large tiles, the columns behind them in smaller ones
+                                        (2300, 7700, 2000, True), (2300, 7700, 2000, False), (4096, 4100, 900, False),
+                                        (4608, 4096, 1400, True), (256, 65_800, 600, True)])
 def test_matmul_of_whole_numbers_is_exact_over_long_sums(require_gpu, m, n, k, pow2):
     """Scales are held for 64 or 256 steps at a time: sums longer than that, exact as above."""
     fp8 = _ops()
@@ -307,6 +310,23 @@ def test_matmul_of_whole_numbers_is_exact_over_long_sums(require_gpu, m, n, k, p
     assert want.abs().max() * 4 < 2 ** 24 and (want * 4 == (want * 4).round()).all()
     got = fp8.matmul(a, b, torch.bfloat16)
     assert torch.equal(got, want.float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("pow2", [False, True])
+@pytest.mark.parametrize("m,n,first", [(2300, 7700, 7168), (4090, 4101, 4096)])
+def test_the_columns_behind_whole_rounds(require_gpu, m, n, first, pow2):
+    """Two kernels share a product: each column as in a product of its part alone, into a wider buffer, with a bias."""
+    fp8 = _ops()
+    k = 900
+    a, b = _matmul_inputs(m, n, k, pow2)
+    bias = _randn((n,), 9, torch.float16).to(DEV)
+    buf = torch.full((m + 2, n + 5), 7.0, dtype=torch.float16, device=DEV)
+    out = fp8.matmul(a, b, torch.float16, bias, buf[1:m + 1, 3:n + 3])
+    for part in (slice(0, first), slice(first, n)):
+        blocks = slice(part.start // 128, -(-part.stop // 128))
+        piece = fp8.BlockMatrix(b.data[part], b.scales[blocks], cols=k, block_rows=128)
+        assert torch.equal(out[:, part], fp8.matmul(a, piece, torch.float16, bias[part]))
+    assert (buf[0] == 7).all() and (buf[-1] == 7).all() and (buf[:, :3] == 7).all() and (buf[:, n + 3:] == 7).all()
 
 
 @pytest.mark.parametrize("pow2", [False, True])
