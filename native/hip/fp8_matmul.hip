@@ -161,7 +161,7 @@ __device__ __forceinline__ void store_tile(const MatArgs& p, const f32x4 (&acc)[
 //   Q1(k)    x0 w1      x1(k)                       w0(k+2)
 //   Q2(k)    x1 w1      x0(k+1)                     w1(k+2)
 //   Q3(k)    x1 w0      w0(k+1), piece by piece     x1(k+2), rows' scales(k+3)
-// A load has six quarters (3072 cycles) to arrive; every wave counts its own loads (4, 4, 4 and 5 a quarter)
+// A load has six quarters (of 512 cycles) to arrive; every wave counts its own loads (4, 4, 4 and 5 a quarter)
 // and waits for those that the quarter reads, and the barrier joins the waits of all four. What a
 // quarter loads into was read a step before (x0: waited for by count at Q0; the others: their
 // products have been issued).
