@@ -84,7 +84,7 @@ __device__ __forceinline__ uint2 to_e4m3(const float (&v)[kWidth], float inv) {
 // A later rounding to fewer bits is then that of the exact value.
 __device__ __forceinline__ float to_odd(float v, float rest) {
   const int b = __float_as_int(v), step = (b ^ __float_as_int(rest)) >> 31 | 1;      // -1 toward 0, 1 away from it
-  return __int_as_float(rest != 0.f && !(b & 1) ? b + step : b);
+  return __int_as_float(fabsf(rest) > 0.f && !(b & 1) ? b + step : b);        // (a NaN rest leaves v as it is)
 }
 
 // The first `keep` of eight bytes, zeros behind them.
@@ -144,6 +144,44 @@ __device__ __forceinline__ void store8(T* row, int c, int cols, const float (&v)
 __device__ __forceinline__ int64_t row_of(int64_t b, int64_t rows) {
   const int64_t run = (rows + kXcds - 1) / kXcds, at = b / kXcds, r = (b % kXcds) * run + at;
   return at < run && r < rows ? r : -1;
+}
+
+// A block of the norm in 64 bits, for what float32 cannot hold on the way: products h * w, a root or values out of
+// (kLeast, kMost), a block of zeros, a row of NaN. (In float32 the factor root / s alone is infinite for a block
+// whose products lie below 2^-119, and its zeros become NaN.) Neither h * w, which is exact, nor root / s leaves
+// 64 bits' range. Returns the scale; all 16 lanes of the block come here together.
+constexpr float kLeast = 1e-30f, kMost = 1e30f;
+
+template <bool POW2>
+__device__ __forceinline__ float wide_block(const float (&h)[kWidth], const float (&w)[kWidth], double root,
+                                            float (&v)[kWidth]) {
+  double amax = 0.;
+#pragma unroll
+  for (int i = 0; i < kWidth; ++i) {
+    const double g = fabs((double)h[i] * w[i]);
+    amax = g <= 1.7976931348623157e308 ? fmax(amax, g) : amax;
+  }
+#pragma unroll
+  for (int off = 1; off < kLanes; off <<= 1) amax = fmax(amax, __shfl_xor(amax, off));
+  amax *= root;                                  // NaN in the row, or 1/0: NaN, scale 1
+  float s = 1.f;
+  if (amax > 0.) {
+    if constexpr (POW2) {
+      const uint64_t b = (uint64_t)__double_as_longlong(amax);
+      const int p = (int)(b >> 52) - 1023 - 8 + ((b & 0xFFFFFFFFFFFFFull) > 0xC000000000000ull);
+      s = __uint_as_float((uint32_t)(min(max(p, -126), 127) + 127) << 23);
+    } else {
+      s = (float)fmin(fmax(amax / 448., 0x1p-126), 3.402823466e38);
+    }
+  }
+  const double f = root / s;
+#pragma unroll
+  for (int i = 0; i < kWidth; ++i) {
+    const double y = (double)h[i] * w[i] * f;
+    v[i] = (float)y;
+    v[i] = to_odd(v[i], (float)(y - v[i]));
+  }
+  return s;
 }
 
 struct NormArgs {
@@ -235,32 +273,41 @@ __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) {
         g[i] = h[i] * w8[i];
-        gmax = fmaxf(gmax, finite_abs(g[i]));
+        gmax = fmaxf(gmax, fabsf(g[i]));               // (NaN counts for nothing)
       }
       gmax = row_max(gmax);
-      float amax = rstd <= 3.402823466e38f ? fminf(gmax * rstd, 3.402823466e38f) : 0.f;   // NaN in the row, or 1/0: NaN, scale 1
-      // a product that was rounded down onto 448 * 2^p lies above it
-      if (POW2 && fmaf(gmax, rstd, -amax) + gmax * rstd_low > 0.f && amax < 3.4e38f)
-        amax = __uint_as_float(__float_as_uint(amax) + 1);
-      const float s = scale_of<POW2>(amax);
-      const float f = rstd * __fdiv_rn(1.f, s), low = rstd_low * __fdiv_rn(1.f, s);
-      // (a scale at its least, and magnitudes that 448 or the inverse would take out of range, go the second way)
-      if (!POW2 && amax > 0.f && s > 1.17549435e-38f && gmax > 1e-30f && gmax < 1e30f) {
-        const float inv = __fdiv_rn(1.f, gmax);
+      if (!(gmax < kMost)) {                           // an infinite weight is left out, a product out of range is not
+        gmax = 0.f;
 #pragma unroll
-        for (int i = 0; i < kWidth; ++i) {
-          const float top = g[i] * 448.f, first = top * inv;
-          const float rest = fmaf(-first, gmax, top);
-          v[i] = fabsf(rest) < 1e30f ? fmaf(rest, inv, first) : first;   // NaN and infinity as they are
-          v[i] = to_odd(v[i], fmaf(-v[i], gmax, top));
+        for (int i = 0; i < kWidth; ++i) gmax = fmaxf(gmax, fabsf(w8[i]) <= 3.402823466e38f ? fabsf(g[i]) : 0.f);
+        gmax = row_max(gmax);
+      }
+      float amax = gmax * rstd;
+      // a product that was rounded down onto 448 * 2^p lies above it
+      if (POW2 && fmaf(gmax, rstd, -amax) + gmax * rstd_low > 0.f) amax = __uint_as_float(__float_as_uint(amax) + 1);
+      float s;
+      if (gmax > kLeast && gmax < kMost && rstd > kLeast && rstd < kMost && amax > kLeast && amax < kMost) {
+        s = scale_of<POW2>(amax);
+        if constexpr (!POW2) {
+          const float inv = __fdiv_rn(1.f, gmax);
+#pragma unroll
+          for (int i = 0; i < kWidth; ++i) {
+            const float top = g[i] * 448.f, first = top * inv;
+            const float rest = fmaf(-first, gmax, top);
+            v[i] = fabsf(rest) < 1e30f ? fmaf(rest, inv, first) : first;   // NaN and infinity as they are
+            v[i] = to_odd(v[i], fmaf(-v[i], gmax, top));
+          }
+        } else {
+          const float f = rstd * __fdiv_rn(1.f, s), low = rstd_low * __fdiv_rn(1.f, s);
+#pragma unroll
+          for (int i = 0; i < kWidth; ++i) {
+            const float rest = g[i] * low;
+            v[i] = fabsf(rest) < 1e30f ? fmaf(g[i], f, rest) : g[i] * f;
+            v[i] = to_odd(v[i], fmaf(g[i], f, -v[i]) + rest);
+          }
         }
       } else {
-#pragma unroll
-        for (int i = 0; i < kWidth; ++i) {
-          const float rest = g[i] * low;
-          v[i] = fabsf(rest) < 1e30f ? fmaf(g[i], f, rest) : g[i] * f;
-          v[i] = to_odd(v[i], fmaf(g[i], f, -v[i]) + rest);
-        }
+        s = wide_block<POW2>(h, w8, root, v);
       }
       uint2 out8 = to_e4m3(v, 1.f);
       if (c + kWidth > a.cols) out8 = clear_past(out8, a.cols - c);      // 0 * NaN in a padded column

@@ -634,3 +634,59 @@ def test_prober_runs_the_matrix_check(require_gpu):
     from yoda_scheduler_amd.sniffer.publisher import HipProber
     wrong, rate = HipProber().matrix(0)
     assert wrong == 0 and rate > 1000
+
+
+@pytest.mark.parametrize("pow2", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("small", [1e-36, 1e-37, 2.0 ** -126, 2.0 ** -133])
+def test_norm_of_a_tiny_block_in_a_normal_row(require_gpu, small, dtype, pow2):
+    """root / s of such a block is beyond float32: its values stay finite, and zeros beside them zeros."""
+    x = (0.02 * _randn((5, 384), 31, spread=0)).to(dtype)
+    x[:, :128] = 0
+    x[0, 3] = small
+    x[1, :128] = small
+    x[2, 0], x[2, 127] = -small, small / 4
+    x[3, 256:] = 0                                                  # tiny beside nothing and something
+    x[3, 5] = small
+    for w in (torch.ones(384, dtype=dtype), (1 + 0.1 * _randn((384,), 32, spread=0)).to(dtype)):
+        q, h = _ops().add_rms_norm(x.to(DEV), w.to(DEV), None, 1e-6, E8M0 if pow2 else torch.float32)
+        assert not q.data.float().isnan().any()
+        _check_norm(q, h, x, w, None, 1e-6, pow2)
+
+
+@pytest.mark.parametrize("pow2", [False, True])
+def test_norm_beyond_what_float32_holds_on_the_way(require_gpu, pow2):
+    """Products h * weight, roots and scales out of float32's range, of values that float32 holds."""
+    sd = E8M0 if pow2 else torch.float32
+    base = _randn((6, 512), 33, spread=0)
+    x, w = base.clone(), torch.ones(512)
+    x[0] *= 2.0 ** 124                                              # h * w beyond 2^128 in the second block
+    x[1] *= 2.0 ** -140                                             # a root beyond it
+    x[2, 128:256] *= 2.0 ** -100                                    # h * w below 2^-149 in the third
+    x[3] *= 2.0 ** 60
+    x[4] = 0
+    w[128:256], w[256:384], w[384:] = 2.0 ** 40, 2.0 ** -100, 2.0 ** -20
+    for eps in (0.0, 1e-300):
+        q, h = _ops().add_rms_norm(x[:4].to(DEV), w.to(DEV), None, eps, sd)
+        _check_norm(q, h, x[:4], w, None, eps, pow2)
+    q, h = _ops().add_rms_norm(x.to(DEV), w.to(DEV), None, 1e-6, sd)
+    _check_norm(q, h, x, w, None, 1e-6, pow2)
+
+
+@pytest.mark.parametrize("infinite", [float("inf"), -float("inf")])
+@pytest.mark.parametrize("pow2", [False, True])
+def test_norm_of_infinities(require_gpu, pow2, infinite):
+    """An infinite weight leaves its column NaN and its block's scale to the others; an infinite value its row."""
+    sd = E8M0 if pow2 else torch.float32
+    x, w = _randn((4, 256), 34, spread=0), torch.ones(256)
+    w[7] = infinite
+    q, _ = _ops().add_rms_norm(x.to(DEV), w.to(DEV), None, 1e-6, sd)
+    got, clean = _dequantized(q), w.clone()
+    clean[7] = 0
+    want, _ = _ops().add_rms_norm(x.to(DEV), clean.to(DEV), None, 1e-6, sd)
+    assert got[:, 7].isnan().all()
+    keep = [i for i in range(256) if i != 7]
+    assert torch.equal(q.scales.float(), want.scales.float()) and torch.equal(got[:, keep], _dequantized(want)[:, keep])
+    x[2, 200] = float("inf")
+    q, _ = _ops().add_rms_norm(x.to(DEV), torch.ones(256, device=DEV), None, 1e-6, sd)
+    assert _dequantized(q)[2, 200].isnan() and not _dequantized(q)[[0, 1, 3]].isnan().any()

@@ -212,9 +212,9 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
 
     Returns (y in e4m3 with 1 × 128 blocks, h); h is None without a residual. ``weight`` [cols] has
     x's type or is float32; x and residual [rows, cols] may have any row stride. Values are the 8-bit ones next to
-    the quotients themselves. Squares are summed in 64 bits, the rest is float32: it holds for rows whose
-    root mean square and products h * weight lie between 2^-100 and 2^120. A row that holds NaN is NaN, and so is
-    one of zeros where eps is 0.
+    the quotients themselves (float32 products h * weight are rounded first). Squares are summed in 64 bits, and so is
+    what float32 does not hold on the way: any finite h and weight will do whose y float32 holds. A row that holds NaN
+    or an infinity has no numbers but zeros, and one of zeros where eps is 0 is NaN.
     """
     pow2 = _scale_kind(scale_dtype)
     got = _native().norm(x, weight, residual, eps, pow2)
