@@ -463,8 +463,7 @@ __global__ __launch_bounds__(512, 2) void k_eight(MatArgs p, int tiles_m, int ti
       const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
       t[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(w[j]), join(x[i & 3]), zero, 0, 0, 0, 0, 0, 0);
       if constexpr (at >= 2) add(Index<at - 2>{});
-      if constexpr (at == 3) meet<9>();
-      if constexpr (at == 19) {
+      if constexpr (at == 3 || at == 19) {          // what is refilled after a meeting has left LDS in every wave
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         meet<9>();
       }
