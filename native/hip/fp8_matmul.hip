@@ -52,21 +52,25 @@ __host__ __device__ __forceinline__ constexpr int column_of(int piece, int c) {
   return (piece >> 1) * 32 + (c >> 2) * 8 + (piece & 1) * 4 + (c & 3);
 }
 
-// Lane l's BYTES at base + voff + soff go to LDS at lds + BYTES * l. (m0 is the compiler's to set before its
-// own uses of it, and it makes none here.)
+// Lane l's BYTES at base + voff + soff go to LDS at lds + BYTES * l. m0 holds lds: the compiler keeps no values of its own
+// in it ("reserved", hence its warning), and the clobber tells it that what it sets there for an instruction of its own
+// does not outlast the load.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int BYTES>
 __device__ __forceinline__ void load_lds(u32x4 rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
   if constexpr (BYTES == 16)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
-                 : "memory");
+                 : "memory", "m0");
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
                  :
                  : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
-                 : "memory");
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 __device__ __forceinline__ u32x4 buffer_of(const void* base) {
   const uint64_t at = (uint64_t)base;

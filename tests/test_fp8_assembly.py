@@ -60,3 +60,14 @@ def test_no_read_of_lds_is_left_where_waves_meet(assembly, kernel, meetings):
             before = loop[:i]
             last = max((j for j, e in enumerate(before) if e != "wait"), default=-1)
             assert "wait" in before[last + 1:], (name, loop)
+
+
+def test_inline_assembly_names_the_register_it_writes():
+    """m0, the direct loads' place in LDS, belongs to the compiler: a statement that sets it says so."""
+    found = 0
+    for path in sorted((build.NATIVE / "hip").glob("*.h*")):
+        for statement in re.findall(r"\basm\s+volatile\s*\((.*?)\);", path.read_text(), re.S):
+            if re.search(r"\bm0, ", statement.partition("\n")[0]):
+                found += 1
+                assert '"m0"' in statement.rpartition(":")[2], (path.name, statement)
+    assert found
