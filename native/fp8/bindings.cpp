@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -34,7 +35,11 @@ int type_of(at::ScalarType t) {
 
 const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
-bool recorded(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// whether a derivative of t is recorded (reverse mode) or goes along with it (forward mode, which no_grad leaves on)
+bool recorded(const at::Tensor& t) {
+  return (at::GradMode::is_enabled() && t.requires_grad()) ||
+         (t._fw_grad(/*level=*/0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode());
+}
 
 // a matrix on a GPU whose columns are neighbours, of a type the operators take, and no part of a graph (a view that
 // negates its values holds others than it shows)
@@ -196,11 +201,12 @@ PyObject* matmul(PyObject*, PyObject* const* args, Py_ssize_t count) {
 }
 
 // corner(t, rows, columns) -> a view of t's first rows and columns, or None where torch has to make it (of a tensor
-// that is part of a graph). A slice in Python takes 2 us, and every call's result is asked for its values and scales.
+// that is part of a graph or has a tangent). A slice in Python takes 2 us, and every call's result is asked for its values and scales.
 PyObject* corner(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   const at::Tensor* t = count == 3 ? tensor(args[0]) : nullptr;
-  if (!t || !t->is_cuda() || t->layout() != at::kStrided || t->dim() != 2 || t->requires_grad() || t->is_inference() || t->is_neg())
+  if (!t || !t->is_cuda() || t->layout() != at::kStrided || t->dim() != 2 || t->requires_grad() || t->_fw_grad(0).defined() ||
+      t->is_inference() || t->is_neg())
     return refused();
   const int64_t rows = PyLong_AsLongLong(args[1]), cols = PyLong_AsLongLong(args[2]);
   if (PyErr_Occurred()) return nullptr;

@@ -161,3 +161,24 @@ def test_matrix_probe_is_off_by_default_and_keeps_to_its_share_of_memory():
     from yoda_scheduler_amd.cmd.sniffer import build_parser
     assert build_parser().parse_args([]).probe_matrix is False
     assert build_parser().parse_args(["--probe", "--probe-matrix"]).probe_matrix is True
+
+
+def test_tangents_are_refused():
+    """A forward-mode tangent would be lost as a gradient would; under no_grad too, which leaves forward mode on."""
+    from torch.autograd import forward_ad
+    x = torch.ones(4, 128)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        b = fp8.BlockMatrix(torch.zeros(4, 128).to(E4M3), forward_ad.make_dual(torch.ones(1, 1), torch.ones(1, 1)),
+                            block_rows=128)
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                fp8._no_grad(None, dual)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                fp8.matmul(_matrix(4, 128), b)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                fp8._no_grad(dual)
+        fp8._no_grad(forward_ad.unpack_dual(dual).primal)
+        with torch.inference_mode():
+            fp8._no_grad(dual)
+    fp8._no_grad(x)

@@ -690,3 +690,28 @@ def test_norm_of_infinities(require_gpu, pow2, infinite):
     x[2, 200] = float("inf")
     q, _ = _ops().add_rms_norm(x.to(DEV), torch.ones(256, device=DEV), None, 1e-6, sd)
     assert _dequantized(q)[2, 200].isnan() and not _dequantized(q)[[0, 1, 3]].isnan().any()
+
+
+def test_tangents_are_refused_on_a_gpu(require_gpu):
+    from torch.autograd import forward_ad
+    fp8 = _ops()
+    x, w = torch.ones(4, 300, device=DEV), torch.ones(300, device=DEV)
+    a, b = _matmul_inputs(4, 200, 300, False)
+    out = torch.zeros(4, 200, device=DEV, dtype=torch.bfloat16)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: fp8.quantize(dual(x)), lambda: fp8.add_rms_norm(dual(x), w),
+                     lambda: fp8.add_rms_norm(x, dual(w)), lambda: fp8.add_rms_norm(x, w, dual(x)),
+                     lambda: fp8.matmul(a, b, bias=dual(torch.zeros(200, device=DEV, dtype=torch.bfloat16))),
+                     lambda: fp8.matmul(a, b, out=dual(out)),
+                     lambda: fp8.matmul(a, fp8.BlockMatrix(b.values, dual(b.scales), block_rows=128))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        q = fp8.quantize(forward_ad.unpack_dual(dual(x)).primal)
+        learned = fp8.BlockMatrix(q.values, dual(q.scales.clone()))
+        assert forward_ad.unpack_dual(learned.scales).tangent is not None        # its views keep it
+        with torch.inference_mode():
+            fp8.quantize(dual(x))

@@ -15,7 +15,7 @@ zeros has scale 1; NaN and infinities become NaN and leave their block's scale a
 
 Every call runs on the current stream of its tensors' device, allocates its outputs with torch,
 waits for nothing and can be captured into a graph. This is the forward path of serving: an input
-that requires a gradient is refused while gradients are recorded.
+that requires a gradient is refused while gradients are recorded, and so is one with a forward-mode tangent.
 """
 from __future__ import annotations
 
@@ -23,6 +23,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import hip
 from .native import load_native
@@ -172,10 +173,13 @@ def _refuse_other(t: torch.Tensor, name: str) -> None:
 
 
 def _no_grad(*tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError("the 8-bit operators have no backward pass: call them under torch.no_grad()")
+    for t in tensors:
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("the 8-bit operators have no backward pass: call them under torch.no_grad()")
+        if forward_ad.unpack_dual(t).tangent is not None:            # (none where forward mode is off)
+            raise RuntimeError("the 8-bit operators have no forward-mode derivative: unpack the dual tensor first")
 
 
 def _scale_kind(dtype: torch.dtype) -> int:
