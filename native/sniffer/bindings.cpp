@@ -12,6 +12,8 @@ using namespace yoda;
 PYBIND11_MODULE(_yoda_sniffer, m) {
   m.def("build_id", [] { return std::string(YODA_BUILD_ID); }, "hash of the sources this module was built from");
   m.doc() = "amd-smi telemetry collector (C++)";
+  m.def("kfd_holders", &kfd_holders, py::arg("proc_root") = "/proc",
+        "{render node: processes that hold it and /dev/kfd open}, as far as this process may look into others");
   py::class_<Collector>(m, "Collector")
       .def(py::init<>())
       .def("init",

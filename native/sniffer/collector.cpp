@@ -4,10 +4,15 @@
 #include <cmath>
 
 #include <amd_smi/amdsmi.h>
+#include <dirent.h>
+#include <unistd.h>
 
 #include <algorithm>
 #include <chrono>
 #include <cstdio>
+#include <cstdlib>
+#include <cstring>
+#include <set>
 #include <sstream>
 #include <tuple>
 
@@ -64,7 +69,38 @@ std::string esc(const std::string& s) {
   return o;
 }
 
+// names in a directory that are numbers (none where it cannot be read)
+std::vector<std::string> numbers_in(const std::string& path) {
+  std::vector<std::string> out;
+  DIR* d = opendir(path.c_str());
+  if (!d) return out;
+  while (const dirent* e = readdir(d))
+    if (e->d_name[0] >= '0' && e->d_name[0] <= '9') out.push_back(e->d_name);
+  closedir(d);
+  return out;
+}
+
 }  // namespace
+
+std::map<int, int> kfd_holders(const std::string& proc_root) {
+  std::map<int, int> out;
+  for (const std::string& pid : numbers_in(proc_root)) {
+    const std::string fds = proc_root + "/" + pid + "/fd/";
+    bool kfd = false;
+    std::set<int> renders;
+    for (const std::string& fd : numbers_in(fds)) {
+      char to[64];
+      const ssize_t n = readlink((fds + fd).c_str(), to, sizeof to - 1);
+      if (n < 0) continue;
+      to[n] = 0;
+      if (!strcmp(to, "/dev/kfd")) kfd = true;
+      else if (!strncmp(to, "/dev/dri/renderD", 16)) renders.insert(atoi(to + 16));
+    }
+    if (kfd)
+      for (int r : renders) ++out[r];
+  }
+  return out;
+}
 
 Collector::~Collector() { shutdown(); }
 
@@ -119,6 +155,9 @@ bool Collector::init(std::string* err) {
 
 std::vector<GpuSample> Collector::sample() {
   std::vector<GpuSample> out;
+  // Without the driver's list amd-smi reports no processes, and success.
+  const bool listed = access("/sys/class/kfd/kfd/proc", R_OK | X_OK) == 0;
+  const std::map<int, int> holders = listed ? std::map<int, int>{} : kfd_holders("/proc");
   for (int i = 0; i < (int)handles_.size(); ++i) {
     auto h = (amdsmi_processor_handle)handles_[i];
     GpuSample g;
@@ -147,7 +186,11 @@ std::vector<GpuSample> Collector::sample() {
       if (kf.current_partition_id != 0xFFFFFFFFu) g.partition_id = (int)kf.current_partition_id;
     }
     uint32_t np = 0;
-    if (amdsmi_get_gpu_process_list(h, &np, nullptr) == AMDSMI_STATUS_SUCCESS ||
+    if (!listed) {
+      const auto it = holders.find(g.drm_render);
+      if (it != holders.end()) g.processes = it->second;
+      g.errors.push_back("process_list");
+    } else if (amdsmi_get_gpu_process_list(h, &np, nullptr) == AMDSMI_STATUS_SUCCESS ||
         np > 0) {
       std::vector<amdsmi_proc_info_t> procs(np + 4);
       uint32_t cap = (uint32_t)procs.size();

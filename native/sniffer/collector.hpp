@@ -45,7 +45,7 @@ struct GpuSample {
   std::string hip_uuid;      // amdsmi_get_gpu_enumeration_info (what ROCR_VISIBLE_DEVICES accepts)
   int hip_id = -1, hsa_id = -1, drm_render = -1, drm_card = -1;
   int kfd_node = -1, partition_id = -1;
-  // tenants: processes with a context on this GPU and the CUs their queues occupy
+  // tenants: processes with a context on this GPU (-1: unknown) and the CUs their queues occupy
   int processes = -1;
   uint32_t proc_cus = 0;     // Σ amdsmi_proc_info_t.cu_occupancy
   uint64_t proc_vram_mb = 0;
@@ -85,6 +85,11 @@ class Collector {
   // previous link counters for rate estimation: (gpu, link) → (t, read, write)
   std::map<std::pair<int, int>, std::tuple<double, uint64_t, uint64_t>> prev_;
 };
+
+// Render node number -> processes that hold it and /dev/kfd open, from the links under proc_root/<pid>/fd. What is left
+// where the driver lists no processes: those of other users and containers cannot be looked into, so a number that is
+// missing here says nothing.
+std::map<int, int> kfd_holders(const std::string& proc_root);
 
 std::string to_json(const std::vector<GpuSample>& s);
 

@@ -1,0 +1,76 @@
+"""Who holds a GPU, where the driver's process list cannot be read, and what the probes make of it (no GPU)."""
+import os
+
+import pytest
+
+from yoda_scheduler_amd.sniffer.collector import FakeBackend, samples_to_scv
+from yoda_scheduler_amd.sniffer.publisher import SnifferAgent
+
+
+class Prober:
+    def __init__(self, backend):
+        self.backend, self.probed = backend, []
+
+    def count(self):
+        return self.backend.count
+
+    def bus_id(self, d):
+        return self.backend._bdf(d)
+
+    def bandwidth_gbps(self, d, nbytes):
+        self.probed.append(d)
+        return 6000.0
+
+    def pattern_errors(self, d, nbytes):
+        return 0
+
+    def matrix_bytes(self):
+        return 1 << 28
+
+    def matrix(self, d):
+        return 0, 2500.0
+
+
+def test_holders_are_found_by_their_open_files(tmp_path):
+    from yoda_scheduler_amd.ops.native import load_native
+    mod = load_native("sniffer", "yoda_scheduler_amd._native._yoda_sniffer")
+
+    def process(pid, *files):
+        d = tmp_path / str(pid) / "fd"
+        d.mkdir(parents=True)
+        for i, f in enumerate(files):
+            os.symlink(f, d / str(i))
+
+    process(10, "/dev/null", "/dev/kfd", "/dev/dri/renderD128")
+    process(11, "/dev/kfd", "/dev/dri/renderD128", "/dev/dri/renderD129", "/dev/dri/renderD129")
+    process(12, "/dev/dri/renderD130")                             # a display, no compute
+    process(13, "/dev/kfd")
+    process(14, "anon_inode:[eventfd]", "/dev/dri/card0" + "x" * 80)
+    (tmp_path / "15").mkdir()                                       # cannot be looked into
+    (tmp_path / "self").mkdir()
+    assert mod.kfd_holders(str(tmp_path)) == {128: 2, 129: 1}
+    assert mod.kfd_holders(str(tmp_path / "none")) == {}
+    assert isinstance(mod.kfd_holders(), dict)
+
+
+@pytest.mark.parametrize("matrix", [False, True])
+def test_a_gpu_whose_processes_are_unknown_is_not_probed(matrix):
+    be = FakeBackend(3, node="n")
+    prober = Prober(be)
+    agent = SnifferAgent(None, "n", be, probe=True, prober=prober, probe_matrix=matrix)
+    s = be.sample()
+    s[0]["processes"] = -1
+    del s[1]["processes"]
+    res = agent.run_probes(s)
+    assert prober.probed == [2] and "unknown" in res[0]["skipped"] and "unknown" in res[1]["skipped"]
+    assert set(agent.probe_skipped) == {0, 1} and 0 not in agent.probe_fail_streak
+    agent.run_probes()                                              # known again
+    assert prober.probed == [2, 0, 1, 2] and not agent.probe_skipped
+
+
+def test_occupancy_is_not_taken_from_a_list_that_could_not_be_read():
+    s = FakeBackend(2, node="n").sample()
+    for x in s:
+        x |= {"processes": 2, "processCUs": 0, "gfxActivity": 70, "errors": ["process_list"]}
+    card = samples_to_scv("n", s).status.card_list[0]
+    assert card.processes == 2 and card.occupancy_source == "gfx-activity" and card.cu_occupancy == 70.0

@@ -177,7 +177,7 @@ def samples_to_scv(node: str, samples: list[dict], interval_ms: int = 1000, meas
         bw = int((measured_bw or {}).get(i, s.get("hbmBandwidthGBps", 0)) or 0)
         cus = int(s.get("computeUnits", 0))
         procs = int(s.get("processes", -1))
-        if procs >= 0 and cus > 0:
+        if procs >= 0 and cus > 0 and "process_list" not in (s.get("errors") or []):
             occ, occ_src = min(100.0, 100.0 * int(s.get("processCUs", 0)) / cus), "process-cus"
         else:
             occ, occ_src = float(s.get("gfxActivity", 0)), "gfx-activity"

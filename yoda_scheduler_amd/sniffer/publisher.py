@@ -12,7 +12,7 @@ one ``PUT .../status`` with the resourceVersion of the previous write (a GET onl
 a 409), so an idle 1000-node cluster costs ~1000/heartbeat writes/s instead of 2000/s.
 
 HBM probes (gfx950 kernels, ``native/hip/probes.hip``) run only on idle GPUs (no tenant
-process and little HBM in use), with a buffer sized from the free HBM, and are repeated
+process, which has to be known, and little HBM in use), with a buffer sized from the free HBM, and are repeated
 every ``probe_interval``; a GPU turns Unhealthy after ``fail_threshold`` consecutive
 failed pattern checks and recovers after a clean one. With ``probe_matrix`` an 8-bit linear
 layer (``native/hip/fp8_probe.hip``) runs after them, checked value by value, and counts
@@ -154,6 +154,10 @@ class SnifferAgent:
                 why = f"busy ({procs} process(es), {used} MB in use)"
                 self.probe_skipped[i] = why
                 res[i] = {"skipped": why}
+                continue
+            if procs < 0:
+                self.probe_skipped[i] = "processes unknown"
+                res[i] = {"skipped": "processes unknown"}
                 continue
             nbytes = min(self.probe_bytes, int(free_mb * self.probe_max_fraction) << 20)
             nbytes -= nbytes % (1 << 20)
