@@ -1,5 +1,8 @@
-"""Who holds a GPU, where the driver's process list cannot be read, and what the probes make of it (no GPU)."""
+"""Who holds a GPU, where the driver's process list cannot be read, what the probes make of it, and their own process."""
 import os
+import signal
+import subprocess
+import sys
 
 import pytest
 
@@ -74,3 +77,53 @@ def test_occupancy_is_not_taken_from_a_list_that_could_not_be_read():
         x |= {"processes": 2, "processCUs": 0, "gfxActivity": 70, "errors": ["process_list"]}
     card = samples_to_scv("n", s).status.card_list[0]
     assert card.processes == 2 and card.occupancy_source == "gfx-activity" and card.cu_occupancy == 70.0
+
+
+def _alone(code):
+    """Run in a process that has loaded nothing yet."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return r.stdout
+
+
+def test_the_agent_keeps_no_context_of_its_own():
+    """Probes run in a process that ends: the agent's own would be on every card from the first probe on, so that the
+    next sample finds them all busy."""
+    out = _alone("from yoda_scheduler_amd.sniffer.publisher import HipProber\n"
+                 "p = HipProber(); print(p.matrix_bytes()); p.close()\n"
+                 "print('libamdhip64' in open('/proc/self/maps').read())")
+    size, mapped = out.split()
+    assert int(size) > 1 << 27 and mapped == "False"
+
+
+def test_a_probing_process_that_fails_hangs_or_ends(monkeypatch):
+    from yoda_scheduler_amd.sniffer import probe
+    w = probe.Worker(timeout=60)
+    with pytest.raises(probe.ProbeError, match="KeyError"):
+        w.ask("nothing of the kind")
+    first = w._child.pid
+    assert w.ask("matrix_bytes") > 0 and w._child.pid == first         # an error is an answer
+    w._child.kill()
+    with pytest.raises(probe.ProbeError, match="ended with status -9"):
+        w.ask("matrix_bytes")
+    assert w.ask("matrix_bytes") > 0 and w._child.pid != first         # and the next question has a new process
+    w.timeout = 0.5
+    os.kill(w._child.pid, signal.SIGSTOP)
+    with pytest.raises(probe.ProbeError, match="ended with status -9"):
+        w.ask("matrix_bytes")
+    w.close()
+    w.close()
+
+
+@pytest.mark.gpu
+def test_probes_leave_no_context_behind(require_gpu):
+    out = _alone("import os\n"
+                 "from yoda_scheduler_amd.sniffer.publisher import HipProber\n"
+                 "p = HipProber()\n"
+                 "print(p.count(), p.bus_id(0), p.bandwidth_gbps(0, 64 << 20) > 100, p.pattern_errors(0, 64 << 20), p.matrix(0)[0])\n"
+                 "p.close()\n"
+                 "links = [os.readlink(f'/proc/self/fd/{f}') for f in os.listdir('/proc/self/fd') if os.path.lexists(f'/proc/self/fd/{f}')]\n"
+                 "print(any('kfd' in x or 'renderD' in x for x in links))")
+    first, second = out.split("\n")[:2]
+    assert first.split()[0] == "1" and first.split()[2:] == ["True", "0", "0"] and second == "False", out

@@ -62,33 +62,35 @@ def hip_to_index(samples: list[dict], hip_count: int, bus_id=None) -> dict[int, 
 
 
 class HipProber:
-    """The gfx950 HBM probes of ``ops.hip`` behind the interface the agent uses."""
+    """The gfx950 probes of ``ops.hip`` behind the interface the agent uses, in a process of their own that ends with
+    :meth:`close` (:mod:`.probe`)."""
+
+    def __init__(self, timeout: float = 120.0) -> None:
+        from .probe import Worker
+        self._worker = Worker(timeout)
 
     def count(self) -> int:
-        from ..ops import hip
-        return hip.device_count()
+        return self._worker.ask("count")
 
     def bus_id(self, d: int) -> str:
-        from ..ops import hip
-        return hip.pci_bus_id(d)
+        return self._worker.ask("bus_id", d)
 
     def bandwidth_gbps(self, d: int, nbytes: int) -> float:
-        from ..ops import hip
-        return float(hip.hbm_bandwidth(d, nbytes, 5)["read_gbps"])
+        return self._worker.ask("bandwidth_gbps", d, nbytes)
 
     def pattern_errors(self, d: int, nbytes: int) -> int:
-        from ..ops import hip
-        return int(hip.hbm_pattern_check(d, nbytes)["errors"])
+        return self._worker.ask("pattern_errors", d, nbytes)
 
     def matrix_bytes(self) -> int:
-        from ..ops import hip
-        return hip.matrix_check_bytes()
+        return self._worker.ask("matrix_bytes")
 
     def matrix(self, d: int) -> tuple[int, float]:
         """(wrong or unstable values, TFLOP/s) of an 8-bit linear layer on the card."""
-        from ..ops import hip
-        r = hip.matrix_check(d)
-        return int(r["errors"]), float(r["tflops"])
+        wrong, rate = self._worker.ask("matrix", d)
+        return wrong, rate
+
+    def close(self) -> None:
+        self._worker.close()
 
 
 class SnifferAgent:
@@ -137,9 +139,17 @@ class SnifferAgent:
     def run_probes(self, samples: Optional[list[dict]] = None) -> dict:
         """Probe every idle GPU once (synchronous; the agent runs it in a worker thread).
         Returns {amd-smi index: result or skip reason}."""
-        prober = self.prober or HipProber()
         if samples is None:
             samples = self.backend.sample()
+        if self.prober is not None:
+            return self._probe_all(self.prober, samples)
+        prober = HipProber()
+        try:
+            return self._probe_all(prober, samples)
+        finally:
+            prober.close()
+
+    def _probe_all(self, prober, samples: list[dict]) -> dict:
         by_index = {int(s["index"]): s for s in samples}
         mapping = hip_to_index(samples, prober.count(), prober.bus_id)
         res: dict = {}
