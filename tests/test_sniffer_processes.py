@@ -127,3 +127,44 @@ def test_probes_leave_no_context_behind(require_gpu):
                  "print(any('kfd' in x or 'renderD' in x for x in links))")
     first, second = out.split("\n")[:2]
     assert first.split()[0] == "1" and first.split()[2:] == ["True", "0", "0"] and second == "False", out
+
+
+class FailingProber(Prober):
+    """Probes of some cards raise, others find errors."""
+
+    def __init__(self, backend, **fails):
+        super().__init__(backend)
+        self.fails = fails                    # what: {card: what it raises or returns}
+
+    def _or(self, what, d, value):
+        v = self.fails.get(what, {}).get(d, value)
+        if isinstance(v, Exception):
+            raise v
+        return v
+
+    def bandwidth_gbps(self, d, nbytes):
+        self.probed.append(d)
+        return self._or("bandwidth", d, 6000.0)
+
+    def pattern_errors(self, d, nbytes):
+        return self._or("pattern", d, 0)
+
+    def matrix(self, d):
+        return self._or("matrix", d, (0, 2500.0))
+
+
+def test_a_probe_that_raises_is_a_failed_one_and_the_rest_counts():
+    be = FakeBackend(4, node="n")
+    prober = FailingProber(be, matrix={0: RuntimeError("hipError 700"), 2: RuntimeError("")}, pattern={0: 7, 1: 9},
+                           bandwidth={3: RuntimeError("no memory")})
+    agent = SnifferAgent(None, "n", be, probe=True, prober=prober, fail_threshold=2, probe_matrix=True)
+    for k in range(2):
+        res = agent.run_probes()
+    assert prober.probed == [0, 1, 2, 3] * 2
+    assert res[0]["pattern_errors"] == 7 and "700" in res[0]["error"] and res[2]["error"] and "no memory" in res[3]["error"]
+    assert [res[i]["fail_streak"] for i in range(4)] == [2] * 4
+    assert {c.health for c in agent.build().status.card_list} == {"Unhealthy"}
+    assert set(agent.measured_bw) == {0, 1, 2} and set(agent.measured_tflops) == {1}
+    prober.fails.clear()
+    agent.run_probes()
+    assert {c.health for c in agent.build().status.card_list} == {"Healthy"}

@@ -176,24 +176,36 @@ class SnifferAgent:
                 res[i] = {"skipped": "too little free HBM"}
                 continue
             self.probe_skipped.pop(i, None)
-            bw = prober.bandwidth_gbps(d, nbytes)
-            errs = prober.pattern_errors(d, nbytes)
-            matrix: dict = {}
-            if self.probe_matrix:
-                # within the fraction of the free HBM that the memory probes keep to
-                if prober.matrix_bytes() > int(free_mb * self.probe_max_fraction) << 20:
-                    matrix = {"matrix_skipped": "too little free HBM"}
-                else:
-                    wrong, tflops = prober.matrix(d)
-                    self.measured_tflops[i] = tflops
-                    matrix = {"matrix_errors": wrong, "matrix_tflops": tflops}
-            self.measured_bw[i] = round(bw)
-            failed = errs or matrix.get("matrix_errors", 0)
+            # a probe that cannot be run to its end is a failed one: what was found before it counts, and so do the
+            # cards behind
+            got: dict = {"hip": d, "bytes": nbytes}
+            try:
+                got["read_gbps"] = prober.bandwidth_gbps(d, nbytes)
+                self.measured_bw[i] = round(got["read_gbps"])
+                got["pattern_errors"] = prober.pattern_errors(d, nbytes)
+            except Exception as e:  # noqa: BLE001
+                got["error"] = str(e) or repr(e)
+            if self.probe_matrix and "error" not in got:
+                got |= self._probe_matrix(prober, d, i, int(free_mb * self.probe_max_fraction) << 20)
+            failed = any(got.get(k) for k in ("error", "pattern_errors", "matrix_errors"))
             self.probe_fail_streak[i] = self.probe_fail_streak.get(i, 0) + 1 if failed else 0
             self.probe_runs[i] = self.probe_runs.get(i, 0) + 1
-            res[i] = {"hip": d, "bytes": nbytes, "read_gbps": bw, "pattern_errors": errs,
-                      "fail_streak": self.probe_fail_streak[i], **matrix}
+            got["fail_streak"] = self.probe_fail_streak[i]
+            res[i] = got
+            if "error" in got:
+                log.warning("GPU %d: probe failed: %s", i, got["error"])
         return res
+
+    def _probe_matrix(self, prober, d: int, i: int, room: int) -> dict:
+        """The matrix check of a card within ``room`` bytes: the fraction of the free HBM that the memory probes keep to."""
+        try:
+            if prober.matrix_bytes() > room:
+                return {"matrix_skipped": "too little free HBM"}
+            wrong, tflops = prober.matrix(d)
+        except Exception as e:  # noqa: BLE001
+            return {"error": str(e) or repr(e)}
+        self.measured_tflops[i] = tflops
+        return {"matrix_errors": wrong, "matrix_tflops": tflops}
 
     async def maybe_probe(self, samples: list[dict]) -> Optional[dict]:
         now = self.clock()
