@@ -168,3 +168,29 @@ def test_a_probe_that_raises_is_a_failed_one_and_the_rest_counts():
     prober.fails.clear()
     agent.run_probes()
     assert {c.health for c in agent.build().status.card_list} == {"Healthy"}
+
+
+def test_a_skipped_matrix_check_clears_no_card_that_it_failed():
+    be = FakeBackend(2, node="n")
+    prober = FailingProber(be, matrix={0: (3, 2500.0)}, pattern={1: 4})
+    agent = SnifferAgent(None, "n", be, probe=True, prober=prober, fail_threshold=2, probe_matrix=True)
+    agent.run_probes()
+    agent.run_probes()
+    assert {c.health for c in agent.build().status.card_list} == {"Unhealthy"}
+    prober.fails.clear()
+    prober.matrix_bytes = lambda: 1 << 50                           # no room: not repeated
+    res = agent.run_probes()
+    assert res[0]["matrix_skipped"] and res[0]["fail_streak"] == 2 and res[1]["fail_streak"] == 0
+    assert [c.health for c in agent.build().status.card_list] == ["Unhealthy", "Healthy"]
+    prober.fails["pattern"] = {0: 1}
+    assert agent.run_probes()[0]["fail_streak"] == 3
+    prober.fails.clear()
+    assert agent.run_probes()[0]["fail_streak"] == 3
+    del prober.matrix_bytes
+    assert agent.run_probes()[0]["fail_streak"] == 0
+    assert {c.health for c in agent.build().status.card_list} == {"Healthy"}
+    # one that raised is a matrix failure as well
+    prober.fails["matrix"] = {1: RuntimeError("hipError 700")}
+    agent.run_probes()
+    prober.matrix_bytes = lambda: 1 << 50
+    assert agent.run_probes()[1]["fail_streak"] == 1

@@ -122,6 +122,7 @@ class SnifferAgent:
         self.probe_fail_streak: dict[int, int] = {}
         self.probe_runs: dict[int, int] = {}
         self.probe_skipped: dict[int, str] = {}
+        self._matrix_failed: set[int] = set()      # cards whose last matrix check failed
         self._last_probe = -1e18
         # publishing state
         self.published = 0
@@ -187,8 +188,12 @@ class SnifferAgent:
                 got["error"] = str(e) or repr(e)
             if self.probe_matrix and "error" not in got:
                 got |= self._probe_matrix(prober, d, i, int(free_mb * self.probe_max_fraction) << 20)
-            failed = any(got.get(k) for k in ("error", "pattern_errors", "matrix_errors"))
-            self.probe_fail_streak[i] = self.probe_fail_streak.get(i, 0) + 1 if failed else 0
+            streak = self.probe_fail_streak.get(i, 0)
+            if any(got.get(k) for k in ("error", "pattern_errors", "matrix_errors")):
+                self.probe_fail_streak[i] = streak + 1
+            else:
+                # a failed matrix check is only cleared by a clean one
+                self.probe_fail_streak[i] = streak if i in self._matrix_failed else 0
             self.probe_runs[i] = self.probe_runs.get(i, 0) + 1
             got["fail_streak"] = self.probe_fail_streak[i]
             res[i] = got
@@ -203,8 +208,10 @@ class SnifferAgent:
                 return {"matrix_skipped": "too little free HBM"}
             wrong, tflops = prober.matrix(d)
         except Exception as e:  # noqa: BLE001
+            self._matrix_failed.add(i)
             return {"error": str(e) or repr(e)}
         self.measured_tflops[i] = tflops
+        (self._matrix_failed.add if wrong else self._matrix_failed.discard)(i)
         return {"matrix_errors": wrong, "matrix_tflops": tflops}
 
     async def maybe_probe(self, samples: list[dict]) -> Optional[dict]:
