@@ -194,3 +194,14 @@ def test_a_skipped_matrix_check_clears_no_card_that_it_failed():
     agent.run_probes()
     prober.matrix_bytes = lambda: 1 << 50
     assert agent.run_probes()[1]["fail_streak"] == 1
+
+
+def test_an_error_of_the_runtime_ends_the_probing_process(monkeypatch):
+    """One card's fault can stay with the process; the next card's probes are not to meet it."""
+    from yoda_scheduler_amd.sniffer import probe
+    w = probe.Worker(timeout=60)
+    with pytest.raises(probe.ProbeError, match="HipError"):
+        w.ask("bus_id", 10 ** 6)
+    assert w._child is None
+    assert w.ask("matrix_bytes") > 0
+    w.close()

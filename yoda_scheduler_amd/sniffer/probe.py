@@ -60,6 +60,8 @@ class Worker:
             raise ProbeError(f"{what}{args}: the probing process ended with status {child.returncode}")
         answer = json.loads(line)
         if "error" in answer:
+            if answer.get("hip"):                     # it may stay with the process: the next card gets a new one
+                self.close()
             raise ProbeError(f"{what}{args}: {answer['error']}")
         return answer["value"]
 
@@ -91,7 +93,7 @@ def main() -> int:
         try:
             answer = {"value": QUESTIONS[what](*args)}
         except Exception as e:  # noqa: BLE001 - said to the one who asked
-            answer = {"error": f"{type(e).__name__}: {e}"}
+            answer = {"error": f"{type(e).__name__}: {e}", "hip": isinstance(e, hip.HipError)}
         print(json.dumps(answer), file=answers, flush=True)
     return 0
 
