@@ -205,3 +205,15 @@ def test_an_error_of_the_runtime_ends_the_probing_process(monkeypatch):
     assert w._child is None
     assert w.ask("matrix_bytes") > 0
     w.close()
+
+
+def test_the_matrix_rate_is_published():
+    from yoda_scheduler_amd.models.scv import Scv
+    be = FakeBackend(2, node="n")
+    prober = FailingProber(be, matrix={1: (0, 40.25)})
+    agent = SnifferAgent(None, "n", be, probe=True, prober=prober, probe_matrix=True)
+    assert "matrixTflops" not in agent.build().to_json()["status"]["amd"]["cards"][0]        # not measured
+    agent.run_probes()
+    obj = agent.build().to_json()
+    assert [c["matrixTflops"] for c in obj["status"]["amd"]["cards"]] == [2500.0, 40.2]
+    assert [c.matrix_tflops for c in Scv.from_json(obj).status.card_list] == [2500.0, 40.2]

@@ -6,7 +6,8 @@ and publishes the node's ``Scv`` status when something the scheduler acts on cha
 (or every ``--heartbeat`` seconds). With ``--probe`` the gfx950 HBM probes run on idle
 GPUs every ``--probe-interval`` seconds (measured bandwidth → ``Card.Bandwidth``,
 ``--probe-fail-threshold`` consecutive pattern failures → ``Card.Health`` Unhealthy);
-``--probe-matrix`` adds a checked 8-bit linear layer on the matrix cores to them.
+``--probe-matrix`` adds a checked 8-bit linear layer on the matrix cores to them (its rate →
+``status.amd.cards[].matrixTflops``).
 ``--print`` samples once and prints the Scv JSON (no apiserver needed).
 """
 from __future__ import annotations

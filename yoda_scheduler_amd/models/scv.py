@@ -61,6 +61,7 @@ _AMD_CARD_FIELDS = {
     "render_node": "renderNode",
     "partition_id": "partitionId",
     "processes": "processes",
+    "matrix_tflops": "matrixTflops",
 }
 
 
@@ -145,6 +146,7 @@ class Card:
     render_node: int = -1       # /dev/dri/renderD<n>
     partition_id: int = -1      # compute partition of a CPX/DPX/QPX logical GPU
     processes: int = -1         # processes with a context on the GPU (-1: unknown)
+    matrix_tflops: float = 0.0  # measured rate of the matrix probe's product (0, and left out: not measured)
 
     @property
     def phys(self) -> int:
@@ -158,6 +160,8 @@ class Card:
         d["physicalId"] = self.phys
         d["id"] = self.id
         d["xgmi"] = [l.to_json() for l in self.xgmi]
+        if not self.matrix_tflops:
+            del d["matrixTflops"]
         return d
 
 

@@ -149,7 +149,8 @@ def _phys_key(bdf: str) -> str:
 
 
 def samples_to_scv(node: str, samples: list[dict], interval_ms: int = 1000, measured_bw: Optional[dict] = None,
-                   probe_errors: Optional[dict] = None, sniffer: str = "amd-smi") -> Scv:
+                   probe_errors: Optional[dict] = None, sniffer: str = "amd-smi",
+                   measured_tflops: Optional[dict] = None) -> Scv:
     """Map one collector sample of every GPU on ``node`` to an ``Scv`` object."""
     phys_ids: dict[str, int] = {}
     for s in samples:
@@ -192,7 +193,8 @@ def samples_to_scv(node: str, samples: list[dict], interval_ms: int = 1000, meas
             ecc_uncorrectable=int(s.get("eccUncorrectable", 0)), xgmi_links_up=int(s.get("xgmiLinksDown", 0)) == 0,
             xgmi=links, uuid=str(s.get("uuid", "")), hip_uuid=str(s.get("hipUuid", "")),
             hip_id=int(s.get("hipId", -1)), render_node=int(s.get("drmRender", -1)),
-            partition_id=int(s.get("partitionId", -1)), processes=procs))
+            partition_id=int(s.get("partitionId", -1)), processes=procs,
+            matrix_tflops=round(float((measured_tflops or {}).get(i, 0.0)), 1)))
     st = ScvStatus(card_list=cards, update_time=max((float(s.get("time", 0)) for s in samples), default=time.time()),
                    sniffer=sniffer)
     st.recompute_sums()

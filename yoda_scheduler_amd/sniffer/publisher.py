@@ -16,7 +16,8 @@ process, which has to be known, and little HBM in use), with a buffer sized from
 every ``probe_interval``; a GPU turns Unhealthy after ``fail_threshold`` consecutive
 failed pattern checks and recovers after a clean one. With ``probe_matrix`` an 8-bit linear
 layer (``native/hip/fp8_probe.hip``) runs after them, checked value by value, and counts
-like a failed pattern check where a value is wrong. Probe results are attributed to
+like a failed pattern check where a value is wrong; its rate is published as the card's
+``matrixTflops``. Probe results are attributed to
 amd-smi indices through the HIP ordinal ↔ amd-smi mapping (``hipId`` from
 ``amdsmi_get_gpu_enumeration_info``, else the PCI bus id), never by assuming the two
 enumerations agree.
@@ -229,7 +230,8 @@ class SnifferAgent:
     def build(self, samples: Optional[list[dict]] = None):
         samples = self.backend.sample() if samples is None else samples
         return samples_to_scv(self.node, samples, int(self.heartbeat * 1000), self.measured_bw or None,
-                              self.probe_unhealthy() or None, sniffer=getattr(self.backend, "name", "amd-smi"))
+                              self.probe_unhealthy() or None, sniffer=getattr(self.backend, "name", "amd-smi"),
+                              measured_tflops=self.measured_tflops or None)
 
     @staticmethod
     def signature(scv) -> tuple:
