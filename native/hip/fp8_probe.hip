@@ -29,6 +29,7 @@ namespace yoda_fp8 {
 namespace {
 
 constexpr double kEps = 1e-6;
+enum Stage { kNorm, kWeight, kProduct, kUnstable, kStages };         // of the counts of wrong values
 
 // about normal (a sum of four uniform values), from the element's place and the seed; bf16
 __global__ __launch_bounds__(256) void k_values(uint16_t* out, int64_t n, uint32_t seed, float scale, float shift) {
@@ -194,7 +195,7 @@ int check(int device, int64_t rows, int64_t cols, int inner, int iters, uint32_t
   void *sa = mem.take(4 * sa_pitch * kb), *sb = mem.take(4 * sb_pitch * (cols / 128));
   const int64_t room = yoda_fp8_matmul_workspace(rows, cols, kb, POW2);
   void* space = mem.take(room + 16);
-  unsigned long long* bad = mem.take<unsigned long long>(8);
+  unsigned long long* bad = mem.take<unsigned long long>(8 * kStages);
   for (hipEvent_t& e : mem.events)
     if (mem.err == hipSuccess) mem.err = hipEventCreate(&e);
   if (mem.err != hipSuccess) return (int)mem.err;
@@ -205,34 +206,39 @@ int check(int device, int64_t rows, int64_t cols, int inner, int iters, uint32_t
   fill(r, xs, seed + 1, 2.f, 0.f);
   fill(gain, inner, seed + 2, 0.1f, 1.f);
   fill(w, ws, seed + 3, small, 0.f);
-  hipError_t e = hipMemset(bad, 0, 8);
+  hipError_t e = hipMemset(bad, 0, 8 * kStages);
   if (e != hipSuccess) return (int)e;
-  int rc = yoda_fp8_norm(device, nullptr, kBf16, 0, POW2, x, inner, r, inner, gain, h, qa, sa, rows, inner, kEps);
-  if (!rc) rc = yoda_fp8_quantize(device, nullptr, kBf16, 1, POW2, w, inner, qb, sb, cols, inner);
+  auto operands = [&] {
+    const int rc = yoda_fp8_norm(device, nullptr, kBf16, 0, POW2, x, inner, r, inner, gain, h, qa, sa, rows, inner, kEps);
+    return rc ? rc : yoda_fp8_quantize(device, nullptr, kBf16, 1, POW2, w, inner, qb, sb, cols, inner);
+  };
+  int rc = operands();
   auto product = [&](uint16_t* to) {
     return yoda_fp8_matmul(device, nullptr, kBf16, POW2, qa, sa, qb, sb, nullptr, to, rows, cols, kb, cols, sa_pitch,
                            room ? space : nullptr, room);
   };
   if (!rc) rc = product(out);
   if (rc) return rc;
-  if (verify_seed != seed) fill(x, xs, verify_seed, 1.f, 0.f), fill(w, ws, verify_seed + 3, small, 0.f);
-  k_check_norm<POW2><<<dim3(kb, (unsigned)rows), 128>>>(x, r, gain, h, qa, sa, sa_pitch, rows, inner, bad);
-  k_check_weight<POW2><<<dim3(kb, (unsigned)(cols / 128)), 256>>>(w, qb, sb, sb_pitch, cols, inner, bad);
+  const bool other = verify_seed != seed;        // the checkers go by another layer: its inputs, and then its operands
+  if (other) fill(x, xs, verify_seed, 1.f, 0.f), fill(w, ws, verify_seed + 3, small, 0.f);
+  k_check_norm<POW2><<<dim3(kb, (unsigned)rows), 128>>>(x, r, gain, h, qa, sa, sa_pitch, rows, inner, bad + kNorm);
+  k_check_weight<POW2><<<dim3(kb, (unsigned)(cols / 128)), 256>>>(w, qb, sb, sb_pitch, cols, inner, bad + kWeight);
+  if (other && (rc = operands())) return rc;
   k_check_product<POW2><<<dim3((unsigned)(cols / 256), (unsigned)rows), 256>>>(qa, sa, sa_pitch, qb, sb, sb_pitch, out, cols,
-                                                                             inner, bad);
+                                                                             inner, bad + kProduct);
   float best = 0.f;
   for (int i = 0; i < iters && !rc; ++i) {       // the same product again: the same bits, and how long it takes
     if ((e = hipEventRecord(mem.events[0], nullptr)) != hipSuccess) return (int)e;
     rc = product(again);
     if ((e = hipEventRecord(mem.events[1], nullptr)) != hipSuccess) return (int)e;
-    k_differ<<<1024, 256>>>((const uint32_t*)out, (const uint32_t*)again, os / 2, bad);
+    k_differ<<<1024, 256>>>((const uint32_t*)out, (const uint32_t*)again, os / 2, bad + kUnstable);
     if ((e = hipEventSynchronize(mem.events[1])) != hipSuccess) return (int)e;
     float ms = 0.f;
     if ((e = hipEventElapsedTime(&ms, mem.events[0], mem.events[1])) != hipSuccess) return (int)e;
     if (i == 0 || ms < best) best = ms;
   }
   if (rc) return rc;
-  if ((e = hipMemcpy(errors, bad, 8, hipMemcpyDeviceToHost)) != hipSuccess) return (int)e;
+  if ((e = hipMemcpy(errors, bad, 8 * kStages, hipMemcpyDeviceToHost)) != hipSuccess) return (int)e;
   *tflops = best > 0.f ? 2. * rows * cols * inner / best / 1e9 : 0.;
   return (int)hipGetLastError();
 }
@@ -252,8 +258,9 @@ int64_t yoda_fp8_matrix_check_bytes(int64_t rows, int64_t cols, int inner) {
 }
 
 // Norm, weight and product of the sizes given (rows from 1 to 65535, cols a multiple of 256, inner of 128), every
-// value checked, the product repeated iters times. *errors: values that are wrong or that changed; *tflops: the
-// fastest product's rate. Returns 0, a hipError, or -1 for sizes out of range.
+// value checked, the product repeated iters times. errors[4]: wrong values of the norm, the weight and the product, and
+// pairs of the product's values that changed; *tflops: the fastest product's rate. With another verify_seed every checker
+// goes by the inputs or operands of that seed's layer and has to find them off. Returns 0, a hipError, or -1 for sizes out of range.
 int yoda_fp8_matrix_check(int device, int64_t rows, int64_t cols, int inner, int iters, int pow2, unsigned seed,
                           unsigned verify_seed, double* tflops, unsigned long long* errors) {
   if (rows < 1 || rows > 65535 || cols < 256 || cols % 256 || cols > (1 << 22) || inner < 128 || inner % 128 ||

@@ -715,3 +715,20 @@ def test_tangents_are_refused_on_a_gpu(require_gpu):
         assert forward_ad.unpack_dual(learned.scales).tangent is not None        # its views keep it
         with torch.inference_mode():
             fp8.quantize(dual(x))
+
+
+@pytest.mark.parametrize("pow2", [False, True])
+def test_each_checker_of_the_matrix_check_compares(require_gpu, pow2):
+    """Checkers that go by another seed's layer find nearly every value of the norm, the weight and the product off,
+    and nearly every pair of values changed in each repetition. Two independent results agree within a checker's
+    bound (a few parts in 2^8 of a value) for a few values in a hundred."""
+    from yoda_scheduler_amd.ops import hip
+    rows, cols, inner, iters = 64, 512, 512, 3
+    keys = ("norm_errors", "weight_errors", "product_errors", "unstable")
+    good = hip.matrix_check(0, rows, cols, inner, iters, pow2, seed=1)
+    assert [good[k] for k in keys] == [0] * 4 and good["errors"] == 0, good
+    bad = hip.matrix_check(0, rows, cols, inner, iters, pow2, seed=1, verify_seed=77)
+    for k, count in zip(keys, (rows * inner, cols * inner, rows * cols, rows * cols // 2 * iters)):
+        # (each of the 256 threads of a block of the weight counts its scale once more)
+        assert 0.8 * count < bad[k] <= count + cols // 128 * (inner // 128) * 256, (k, bad)
+    assert bad["errors"] == sum(bad[k] for k in keys)

@@ -153,17 +153,18 @@ def matrix_check(device: int = 0, rows: int = 4096, cols: int = 4096, inner: int
                  pow2: bool = True, seed: int = 0x5eed, verify_seed: int | None = None) -> dict:
     """Run an 8-bit linear layer of the sizes given (:mod:`.fp8`: residual + norm, a weight's blocks, their
     product), check every value against plain vector code and time the product. ``errors`` counts
-    values that are wrong or that change from one repetition to the next; ``verify_seed`` ≠ ``seed`` is the
-    checkers' self-test (the norm's and the weight's values must mismatch)."""
-    rate, err = c_double(0), c_ull(0)
+    values that are wrong (``norm_errors``, ``weight_errors``, ``product_errors``) and pairs of the product's values
+    that change from one repetition to the next (``unstable``); ``verify_seed`` ≠ ``seed`` is the
+    checkers' self-test (nearly all of each must mismatch)."""
+    rate, err = c_double(0), (c_ull * 4)()
     vs = seed if verify_seed is None else verify_seed
-    rc = lib().yoda_fp8_matrix_check(device, rows, cols, inner, iters, int(pow2), seed, vs, ctypes.byref(rate),
-                                     ctypes.byref(err))
+    rc = lib().yoda_fp8_matrix_check(device, rows, cols, inner, iters, int(pow2), seed, vs, ctypes.byref(rate), err)
     if rc < 0:
         raise ValueError(f"matrix_check: {rows} rows (1 to 65535), {cols} columns (a multiple of 256) and {inner} "
                          "inner (a multiple of 128) are out of range")
     _check(rc, "matrix_check")
-    return {"errors": err.value, "tflops": rate.value, "rows": rows, "cols": cols, "inner": inner, "iters": iters,
+    return {"errors": sum(err), "norm_errors": err[0], "weight_errors": err[1], "product_errors": err[2],
+            "unstable": err[3], "tflops": rate.value, "rows": rows, "cols": cols, "inner": inner, "iters": iters,
             "values": rows * inner + cols * inner + rows * cols}
 
 
