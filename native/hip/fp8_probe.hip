@@ -2,7 +2,7 @@
 // by value against plain vector code and timed. What the HBM probes do not reach: matrix instructions, 8-bit
 // conversions, LDS and the loads into it. A card that computes wrongly there passes every memory check.
 //
-// The checkers share no code with the operators: one thread sums a value from its definition, in float64
+// The checkers share no arithmetic with the operators: one thread sums a value from its definition, in float64
 // for the norm and the weight, and for the product with the bound that the operator's sums have (each
 // eight neighbouring products lose less than 7 * 2^-13 of their largest; then float32, then bf16).
 //
@@ -43,6 +43,13 @@ __global__ __launch_bounds__(256) void k_values(uint16_t* out, int64_t n, uint32
   }
 }
 
+// v to bf16, to nearest, ties to even, by whole numbers (the operators convert by an instruction)
+__device__ uint16_t round_bf16(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return (uint16_t)((b + 0x7FFF + (b >> 16 & 1)) >> 16);
+}
+
+__device__ double bf16(uint16_t v) { return (double)__uint_as_float((uint32_t)v << 16); }
 __device__ double bf16(const uint16_t* p, int64_t i) { return (double)__uint_as_float((uint32_t)p[i] << 16); }
 
 __device__ double e4m3(uint8_t b) {
@@ -87,7 +94,7 @@ __global__ __launch_bounds__(128) void k_check_norm(const uint16_t* x, const uin
   double sum = 0;
   for (int k = t; k < cols; k += 128) {
     const float v = (float)bf16(x, m * cols + k) + (float)bf16(r, m * cols + k);
-    const double b = (double)load_f32<__hip_bfloat16>(store_bits<__hip_bfloat16>(v));
+    const double b = bf16(round_bf16(v));
     sum += b * b;
   }
   part[t] = sum;
@@ -96,8 +103,8 @@ __global__ __launch_bounds__(128) void k_check_norm(const uint16_t* x, const uin
   for (int i = 0; i < 128; ++i) sum += part[i];
   __syncthreads();
   const float v = (float)bf16(x, m * cols + c) + (float)bf16(r, m * cols + c);
-  const uint16_t hb = store_bits<__hip_bfloat16>(v);
-  const double y = (double)load_f32<__hip_bfloat16>(hb) / sqrt(sum / cols + kEps) * bf16(gain, c);
+  const uint16_t hb = round_bf16(v);
+  const double y = bf16(hb) / sqrt(sum / cols + kEps) * bf16(gain, c);
   part[t] = fabs(y);
   __syncthreads();
   double amax = 0;
