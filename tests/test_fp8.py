@@ -182,3 +182,21 @@ def test_tangents_are_refused():
         with torch.inference_mode():
             fp8._no_grad(dual)
     fp8._no_grad(x)
+
+
+def test_another_torch_makes_the_module_stale(tmp_path, monkeypatch):
+    """The module is compiled against torch's C++ internals: its build id names the torch it was built with."""
+    from yoda_scheduler_amd.ops import build
+
+    def ids(where, version):
+        d = tmp_path / where
+        d.mkdir(exist_ok=True)
+        (d / "version.py").write_text(f"__version__ = '{version}'\n")
+        monkeypatch.setattr(build, "torch_root", lambda: d)
+        return build.source_hash("fp8"), build.source_hash("hip")
+
+    here, other, moved = ids("a", "2.10.0"), ids("a", "2.11.0"), ids("b", "2.10.0")
+    assert len({here[0], other[0], moved[0]}) == 3 and here[1] == other[1] == moved[1]
+    assert ids("a", "2.10.0") == here
+    monkeypatch.setattr(build, "torch_root", lambda: None)
+    assert build.source_hash("fp8") not in (here[0], other[0], moved[0])

@@ -16,7 +16,8 @@ Outputs land in ``yoda_scheduler_amd/_native/`` so they travel with the repo sna
 to the GPU box.
 
 Build provenance: each artefact's identity is :func:`source_hash` — a hash of its source
-files' contents (relative paths + bytes) and its compile recipe. It is compiled in
+files' contents (relative paths + bytes) and its compile recipe, and for ``_yoda_fp8`` of the
+torch it is compiled against. It is compiled in
 (``-DYODA_BUILD_ID``: ``build_id()`` of the pybind modules, ``yoda_build_id()`` of the HIP
 library, ``--build-id`` of the binaries) and written next to the artefact
 (``<artefact>.buildid``). A rebuild happens when that hash changes — not on mtimes, which a
@@ -104,7 +105,18 @@ def source_hash(name: str, native: Path | None = None) -> str:
         p = native / rel
         h.update(b"\0" + rel.encode() + b"\0")
         h.update(p.read_bytes() if p.exists() else b"<missing>")
+    if name == "fp8":
+        h.update(_torch_identity())
     return h.hexdigest()[:16]
+
+
+def _torch_identity() -> bytes:
+    """The torch whose C++ internals ``_yoda_fp8`` is compiled against and finds by its path."""
+    torch = torch_root()
+    if torch is None:
+        return b"<no torch>"
+    version = torch / "version.py"
+    return str(torch).encode() + b"\0" + (version.read_bytes() if version.exists() else b"<missing>")
 
 
 def out_path(name: str) -> Path:
@@ -245,8 +257,11 @@ def build_fp8(force: bool = False) -> list[Path]:
         inc = [f"-I{torch / 'include'}", f"-I{torch / 'include/torch/csrc/api/include'}",
                f"-I{sysconfig.get_paths()['include']}", f"-I{NATIVE / 'common'}", f"-I{ROCM / 'include'}",
                "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"]
+        # (in a process of its own: one that loads libyoda_hip.so first may not import torch afterwards)
+        abi = subprocess.run([sys.executable, "-c", "import torch; print(int(torch.compiled_with_cxx11_abi()))"],
+                             capture_output=True, text=True, check=True).stdout.split()[-1]
         _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
-              "-Wno-unused-function", "-D_GLIBCXX_USE_CXX11_ABI=1", _bid_flag(bid), *inc, *_srcs("fp8"), "-o", str(out),
+              "-Wno-unused-function", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", _bid_flag(bid), *inc, *_srcs("fp8"), "-o", str(out),
               f"-L{torch / 'lib'}", f"-Wl,-rpath,{torch / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python"],
              "8-bit operators' torch module")
         _record("fp8", bid)
