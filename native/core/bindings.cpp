@@ -620,6 +620,7 @@ PYBIND11_MODULE(_yoda_core, m) {
                    if (t[1].is_none() || py::len(t[1]) == 0) x.ns.push_back(r.ns);
                    else
                      for (auto n : t[1]) x.ns.push_back(e.intern(n.cast<std::string>()));
+                   x.unique_ns();
                    x.sel = lsel_of(e, t[2]);
                    x.weight = t[3].cast<int32_t>();
                    dst[k]->push_back(std::move(x));

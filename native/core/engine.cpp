@@ -2006,11 +2006,8 @@ int64_t Engine::group_count(const Node& n, int32_t ns, const LSel& sel, bool ski
 int64_t Engine::term_count(const Node& n, const PodTerm& t) const {
   int64_t sum = 0, c = 0;
   bool ok = true;
-  // a namespace that a term names twice counts once
-  auto again = [&](size_t i) { return std::find(t.ns.begin(), t.ns.begin() + i, t.ns[i]) != t.ns.begin() + i; };
-  for (size_t i = 0; i < t.ns.size(); ++i) {
-    if (again(i)) continue;
-    if (!indexed_count(n, t.ns[i], t.sel, false, &c)) {
+  for (int32_t ns : t.ns) {
+    if (!indexed_count(n, ns, t.sel, false, &c)) {
       ok = false;
       break;
     }
@@ -2018,8 +2015,7 @@ int64_t Engine::term_count(const Node& n, const PodTerm& t) const {
   }
   if (ok) return sum;
   sum = 0;
-  for (size_t i = 0; i < t.ns.size(); ++i)
-    if (!again(i)) sum += group_count(n, t.ns[i], t.sel, false);
+  for (int32_t ns : t.ns) sum += group_count(n, ns, t.sel, false);
   return sum;
 }
 

@@ -138,9 +138,13 @@ struct SpreadC {
 // namespaces it selects pods in (the owner's own when the term lists none) and the selector
 struct PodTerm {
   int32_t key = 0;
-  std::vector<int32_t> ns;
+  std::vector<int32_t> ns;     // in order, each once (unique_ns): a namespace that a term names twice counts once
   LSel sel;
   int32_t weight = 1;          // preferred terms
+  void unique_ns() {
+    std::sort(ns.begin(), ns.end());
+    ns.erase(std::unique(ns.begin(), ns.end()), ns.end());
+  }
   bool matches(int32_t pod_ns, const Labels& l) const {
     return std::find(ns.begin(), ns.end(), pod_ns) != ns.end() && sel.matches(l);
   }

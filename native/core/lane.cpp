@@ -1091,6 +1091,7 @@ bool Lane::make_req(const yk::PodProj& p, PodReq* r) {
         x.key = eng_->intern(t.key);
         if (t.ns.empty()) x.ns.push_back(r->ns);
         for (const auto& n : t.ns) x.ns.push_back(eng_->intern(n));
+        x.unique_ns();
         x.sel.nothing = !t.has_sel;
         for (const auto& kv : t.labels) x.sel.reqs.push_back(LReq{eng_->intern(kv.first), kIn, {eng_->intern(kv.second)}});
         for (const auto& q : t.exprs) {

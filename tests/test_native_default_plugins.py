@@ -826,3 +826,35 @@ def test_csi_limits_skip_a_driver_the_pod_adds_no_volume_to():
         eng.set_req_claims(req, pvc_claim_keys(p), True)
         assert pl.filter(CycleState(), p, "n0").is_success() == want, claim
         assert (eng.filter_node(req, eng.node_index("n0")) == 0) == want, claim
+
+
+def test_scoring_grows_with_a_terms_namespaces_and_not_with_their_square():
+    """What a term's repeated namespaces cost is paid when the term is read, not on each node: four times the
+    namespaces are four times the lookups (sixteen times where each is sought among those before it)."""
+    import time
+    from yoda_scheduler_amd.models.device import make_scv
+    from yoda_scheduler_amd.ops.native import push_scv
+    eng = C.Engine(False, 1)
+    nodes = 40
+    for i in range(nodes):
+        idx = eng.upsert_node(f"n{i}")
+        eng.set_node_meta(idx, False, [(HOST, f"n{i}")], [], 192000, 2 << 40, 110)
+        push_scv(eng, idx, make_scv(f"n{i}"), compat=False)
+    for i in range(nodes):
+        assert eng.schedule(i + 1, pod_req(eng, pod(f"q{i}", {"app": "w"})), True)[0] >= 0
+    only_weight(eng, C.S_INTERPOD)
+
+    def least(count, of=5):
+        term = {"topologyKey": HOST, "namespaces": [f"ns{k}" for k in range(count)],
+                "labelSelector": {"matchLabels": {"app": "w"}}}
+        p = pod("new", affinity={"podAntiAffinity": {"preferredDuringSchedulingIgnoredDuringExecution": [
+            {"weight": 5, "podAffinityTerm": term}]}})
+        req, took = pod_req(eng, p), []
+        for _ in range(of):
+            t = time.perf_counter()
+            eng.score_nodes(req, list(range(nodes)))
+            took.append(time.perf_counter() - t)
+        return min(took)
+
+    least(1000)
+    assert min(least(4000) / least(1000) for _ in range(3)) < 9
