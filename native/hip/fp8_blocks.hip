@@ -197,8 +197,10 @@ struct NormArgs {
 //
 // Many rows: HBM. 16384 x 8192 in bf16 with a residual stream moves 940 MB in 186 us, 5.05 TB/s where a copy of 1 GB
 // reaches 5.12; 512 or 1024 lanes a row, non-temporal loads and stores, and 32-bit sums were no faster.
-// Few rows: the way of one row through load, sum, barrier, weight and store. Twice the lanes take
-// 1 x 4096 from 4.5 to 3.6 us, 333 x 5001 from 6.4 to 5.6 and 64 x 8192 from 7.3 to 5.1 up to 1024 rows
+// Few rows: the way of one row through load, sum, barrier, weight and store. From a graph, without a residual: 1 x 4096 3.1 us, 333 x 5001 5.3 on the same
+// rows again and 7.1 on new ones (333 x 5120 4.9 and 6.6, 64 x 8192 4.4 and 5.0): what it takes beyond one row's is the
+// way to memory, for two workgroups on a CU. Twice the lanes took 1 x 4096 with a residual from 4.5 to 3.6 us, 333 x 5001
+// from 6.4 to 5.6 and 64 x 8192 from 7.3 to 5.1 up to 1024 rows
 // (four a CU); with more they cost 3 % (4096 x 4096 30.7 : 31.3) to 5 % (2000 x 5001 14.6 : 15.3).
 template <typename T, typename W, bool POW2, bool RES, int THREADS, int CHUNKS>
 __global__ __launch_bounds__(THREADS) void k_norm(NormArgs a) {

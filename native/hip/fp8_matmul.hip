@@ -170,10 +170,10 @@ __device__ __forceinline__ void store_tile(const MatArgs& p, const f32x4 (&acc)[
 // quarter loads into was read a step before (x0: waited for by count at Q0; the others: their
 // products have been issued).
 //
-// 8192 x 8192 x 8192: 393 to 398 us, 2.8 PFLOP/s (a library's product with one scale for each matrix: 355 us), 4096 x 4096 x
-// 4096: 53 us. The matrix units are busy 72 % of the time at 1.93 GHz, to which the card's power holds the
-// clock (at 84 % the library runs at 1.76). Per step the reads and loads take as long in LDS as the products: with no
-// loads 358 us, with no reads 346, with neither 306. Two meetings a step, 2, 8 or 16 rows of tiles a column and
+// 8192 x 8192 x 8192: 381 to 404 us by card, 2.7 to 2.9 PFLOP/s (a library's product with one scale for each matrix: 355
+// us), 4096 x 4096 x 4096: 53 to 55 us. The matrix units are busy 69 to 72 % of the time, at 1.93 GHz (the library's 84 %,
+// at 1.76): the busier they are, the lower the card's clock. A step's reads and loads are 1536 cycles of LDS beside the 2048
+// of its products. Two meetings a step, 2, 8 or 16 rows of tiles a column and
 // non-temporal stores were no faster. The stores of a round of tiles are 5 us of the 100, at the memory's rate.
 struct Quarters {
   static constexpr int BM = 256, BN = 256;
@@ -345,7 +345,7 @@ __global__ __launch_bounds__(256, 1) void k_quarters(MatArgs p, int tiles_m, int
 //   after the second          rows' pieces 4-7 (k+2), rows' scales (k+3)
 // so a load has a step and a half to arrive. Each wave counts its own loads: 6 and 3.
 //
-// 4096 x 4096 x 4096: 59 to 61 us, 2.3 PFLOP/s, the matrix units busy 64 % of the time; 8192 x 8192 x 8192: 446 to 450.
+// 4096 x 4096 x 4096: 58 to 61 us, 2.3 PFLOP/s, the matrix units busy 62 to 64 % of the time; 8192 x 8192 x 8192: 446 to 450.
 // Bound as k_quarters is, with 192 KB a step read from LDS instead of
 // 128: e8m0 scales take 53 us. (Four waves of 128 x 128 would hold 256 sums a lane, which leaves
 // no vector registers for the multiply-adds.)
@@ -863,6 +863,8 @@ int narrow(const MatArgs& p, bool pow2, hipStream_t s) {
 //   small tiles     up to 256 workgroups 5 + `one` a step, else 2 + (`round` + `two` a step) a round of 512, and no
 //                   less than 3 + weight / 5.3 MB; K in parts: 2.5 more, and twice the parts' bytes / 5 MB
 //   256 x 256       (10.5 + 1.4 a step, float scales 1.57) a round of 256; a last round of a share f counts (1 + f) / 2
+// (They order the kinds; a time itself may be off by a quarter: 777 x 5000 x 1928 comes out as 21 us and takes 17, few rows
+// times few columns, whose workgroups are too few to draw the card's whole rate, as less than they take.)
 // Measured, this one : the next best, e8m0 scales: 16 x 8192 x 8192 few rows 13.4 : 14.9 32 x 32;
 // 32 x 8192 x 8192 32 x 32 14.7 : 16.1 64 x 32; 64 x 8192 x 8192 64 x 32 15.3 : 16.7 64 x 64; 128 x 8192 x 4096 128 x 32
 // 12 : 15 128 x 128 in two parts; 2048 x 2048 x 4096 128 x 128 23 : 44 256 x 256; 4096 x 4096 x 4096 256 x 256
