@@ -105,12 +105,12 @@ def test_a_probing_process_that_fails_hangs_or_ends(monkeypatch):
     first = w._child.pid
     assert w.ask("matrix_bytes") > 0 and w._child.pid == first         # an error is an answer
     w._child.kill()
-    with pytest.raises(probe.ProbeError, match="ended with status -9"):
+    with pytest.raises(probe.ProbeError, match="ended .status -9"):
         w.ask("matrix_bytes")
     assert w.ask("matrix_bytes") > 0 and w._child.pid != first         # and the next question has a new process
     w.timeout = 0.5
     os.kill(w._child.pid, signal.SIGSTOP)
-    with pytest.raises(probe.ProbeError, match="ended with status -9"):
+    with pytest.raises(probe.ProbeError, match="no answer in 0.5 s"):
         w.ask("matrix_bytes")
     w.close()
     w.close()
@@ -217,3 +217,29 @@ def test_the_matrix_rate_is_published():
     obj = agent.build().to_json()
     assert [c["matrixTflops"] for c in obj["status"]["amd"]["cards"]] == [2500.0, 40.2]
     assert [c.matrix_tflops for c in Scv.from_json(obj).status.card_list] == [2500.0, 40.2]
+
+
+def test_a_probing_process_that_cannot_be_killed_is_left(monkeypatch):
+    """One that hangs in the driver outlives a kill and holds its pipes: the agent goes on."""
+    from yoda_scheduler_amd.sniffer import probe
+
+    class Hung:
+        returncode = None
+
+        def __init__(self, *args, **kw):
+            out, self.held = os.pipe()
+            into, give = os.pipe()
+            self.stdout, self.stdin, self.read = os.fdopen(out), os.fdopen(give, "w"), into
+            self.kills = 0
+
+        def kill(self):
+            self.kills += 1
+
+        def wait(self, timeout):
+            raise subprocess.TimeoutExpired("hung", timeout)
+
+    monkeypatch.setattr(probe.subprocess, "Popen", Hung)
+    w = probe.Worker(timeout=0.2)
+    with pytest.raises(probe.ProbeError, match="no answer in 0.2 s"):
+        w.ask("matrix", 0)
+    assert w._child is None

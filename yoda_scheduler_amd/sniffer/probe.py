@@ -9,9 +9,9 @@ from __future__ import annotations
 
 import json
 import os
+import select
 import subprocess
 import sys
-import threading
 from pathlib import Path
 from typing import Any, Optional
 
@@ -45,19 +45,21 @@ class Worker:
             self._child = subprocess.Popen([sys.executable, "-m", __name__], stdin=subprocess.PIPE,
                                            stdout=subprocess.PIPE, text=True, env=env)
         child = self._child
-        late = threading.Timer(self.timeout, child.kill)
-        late.start()
+        line, why = "", "the probing process ended"
         try:
             child.stdin.write(json.dumps([what, *args]) + "\n")
             child.stdin.flush()
-            line = child.stdout.readline()
+            # (an answer is one write of one line)
+            if select.select([child.stdout], [], [], self.timeout)[0]:
+                line = child.stdout.readline()
+            else:
+                why = f"no answer in {self.timeout:g} s, the probing process was killed"
+                child.kill()
         except OSError:
-            line = ""
-        finally:
-            late.cancel()
+            pass
         if not line:
             self.close()
-            raise ProbeError(f"{what}{args}: the probing process ended with status {child.returncode}")
+            raise ProbeError(f"{what}{args}: {why} (status {child.returncode})")
         answer = json.loads(line)
         if "error" in answer:
             if answer.get("hip"):                     # it may stay with the process: the next card gets a new one
@@ -73,11 +75,12 @@ class Worker:
             child.stdin.close()
         except OSError:
             pass
-        try:
-            child.wait(self.timeout)
-        except subprocess.TimeoutExpired:
-            child.kill()
-            child.wait()
+        for _ in range(2):
+            try:
+                child.wait(10.0)
+                break
+            except subprocess.TimeoutExpired:          # after a kill: it hangs in the driver, and is left to it
+                child.kill()
         child.stdout.close()
 
     def __del__(self) -> None:
