@@ -732,3 +732,8 @@ def test_each_checker_of_the_matrix_check_compares(require_gpu, pow2):
         # (each of the 256 threads of a block of the weight counts its scale once more)
         assert 0.8 * count < bad[k] <= count + cols // 128 * (inner // 128) * 256, (k, bad)
     assert bad["errors"] == sum(bad[k] for k in keys)
+
+
+def test_float_scales_held_beyond_256_steps(require_gpu):
+    """Large tiles with float scales take up the columns' scales of 256 steps at a time: exact whole numbers over more."""
+    test_matmul_of_whole_numbers_is_exact_over_long_sums(None, 2900, 3900, 66_000, False)
