@@ -243,3 +243,33 @@ def test_a_probing_process_that_cannot_be_killed_is_left(monkeypatch):
     with pytest.raises(probe.ProbeError, match="no answer in 0.2 s"):
         w.ask("matrix", 0)
     assert w._child is None
+
+
+@pytest.mark.parametrize("said", ["", "{\\\"value", "{}"])
+def test_an_answer_that_is_cut_off_is_none(monkeypatch, said):
+    from yoda_scheduler_amd.sniffer import probe
+    real = subprocess.Popen
+    monkeypatch.setattr(probe.subprocess, "Popen", lambda cmd, **kw: real(["sh", "-c", f'read q; printf "{said}"'], **kw))
+    w = probe.Worker(timeout=60)
+    with pytest.raises(probe.ProbeError, match="the probing process ended .status 0"):
+        w.ask("matrix", 0)
+
+
+def test_an_answer_reaches_a_process_with_many_open_files():
+    """More than select() counts to."""
+    import resource
+    from yoda_scheduler_amd.sniffer import probe
+    soft, hard = resource.getrlimit(resource.RLIMIT_NOFILE)
+    if hard != resource.RLIM_INFINITY and hard < 2048:
+        pytest.skip("few files allowed")
+    resource.setrlimit(resource.RLIMIT_NOFILE, (2048, hard))
+    held = []
+    try:
+        held = [os.open("/dev/null", os.O_RDONLY) for _ in range(1100)]
+        w = probe.Worker(timeout=60)
+        assert w.ask("matrix_bytes") > 0
+        w.close()
+    finally:
+        for fd in held:
+            os.close(fd)
+        resource.setrlimit(resource.RLIMIT_NOFILE, (soft, hard))

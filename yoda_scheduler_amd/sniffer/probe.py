@@ -50,14 +50,16 @@ class Worker:
             child.stdin.write(json.dumps([what, *args]) + "\n")
             child.stdin.flush()
             # (an answer is one write of one line)
-            if select.select([child.stdout], [], [], self.timeout)[0]:
+            ready = select.poll()
+            ready.register(child.stdout, select.POLLIN)
+            if ready.poll(self.timeout * 1000):
                 line = child.stdout.readline()
             else:
                 why = f"no answer in {self.timeout:g} s, the probing process was killed"
                 child.kill()
         except OSError:
             pass
-        if not line:
+        if not line.endswith("\n"):                    # nothing, or cut off
             self.close()
             raise ProbeError(f"{what}{args}: {why} (status {child.returncode})")
         answer = json.loads(line)
