@@ -273,3 +273,27 @@ def test_an_answer_reaches_a_process_with_many_open_files():
         for fd in held:
             os.close(fd)
         resource.setrlimit(resource.RLIMIT_NOFILE, (soft, hard))
+
+
+def test_an_error_that_says_nothing_about_the_card_counts_for_nothing():
+    """No memory (a tenant was quicker) and a fault of the program leave a card's failures as they are."""
+    from yoda_scheduler_amd.ops.hip import HipError
+    from yoda_scheduler_amd.sniffer import probe
+    be = FakeBackend(4, node="n")
+    prober = FailingProber(be, matrix={0: probe.ProbeError("AttributeError: no operators", of_card=False),
+                                       1: probe.ProbeError("the probing process ended")},
+                           pattern={2: probe.ProbeError("hipError 2", of_card=False)})
+    agent = SnifferAgent(None, "n", be, probe=True, prober=prober, fail_threshold=2, probe_matrix=True)
+    agent.run_probes()
+    res = agent.run_probes()
+    assert all("error" in res[i] for i in (0, 1, 2))
+    assert [res[i]["fail_streak"] for i in range(4)] == [0, 2, 0, 0]
+    prober.fails = {"matrix": {1: probe.ProbeError("hipError 2", of_card=False)}}
+    assert agent.run_probes()[1]["fail_streak"] == 2                   # neither cleared nor counted
+    assert HipError("x").code == 0
+    w = probe.Worker(timeout=60)
+    for what, args, of_card in (("nothing of the kind", (), False), ("bus_id", (10 ** 6,), True)):
+        with pytest.raises(probe.ProbeError) as e:
+            w.ask(what, *args)
+        assert e.value.of_card is of_card
+    w.close()

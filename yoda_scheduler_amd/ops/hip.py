@@ -28,7 +28,11 @@ c_int, c_uint, c_ull, c_int64, c_double, c_float, c_char_p, c_void_p = (
 
 
 class HipError(RuntimeError):
-    pass
+    """A call of the HIP runtime that failed; ``code`` is its hipError_t (0: not said)."""
+
+    def __init__(self, message: str, code: int = 0) -> None:
+        super().__init__(message)
+        self.code = code
 
 
 def _declare(lib: ctypes.CDLL) -> None:
@@ -101,7 +105,7 @@ def build_id(l: Optional[ctypes.CDLL] = None) -> str:
 
 def _check(rc: int, what: str) -> None:
     if rc != 0:
-        raise HipError(f"{what} failed with hipError {rc}")
+        raise HipError(f"{what} failed with hipError {rc}", rc)
 
 
 def device_count() -> int:

@@ -27,8 +27,15 @@ QUESTIONS = {
 }
 
 
+_OUT_OF_MEMORY = 2                    # hipErrorOutOfMemory: a tenant was quicker
+
+
 class ProbeError(RuntimeError):
-    """A probe that could not be run to its end."""
+    """A probe that could not be run to its end; ``of_card``: for all that is known, because of the card."""
+
+    def __init__(self, message: str, of_card: bool = True) -> None:
+        super().__init__(message)
+        self.of_card = of_card
 
 
 class Worker:
@@ -64,9 +71,9 @@ class Worker:
             raise ProbeError(f"{what}{args}: {why} (status {child.returncode})")
         answer = json.loads(line)
         if "error" in answer:
-            if answer.get("hip"):                     # it may stay with the process: the next card gets a new one
+            if answer["hip"]:                         # it may stay with the process: the next card gets a new one
                 self.close()
-            raise ProbeError(f"{what}{args}: {answer['error']}")
+            raise ProbeError(f"{what}{args}: {answer['error']}", of_card=answer["of_card"])
         return answer["value"]
 
     def close(self) -> None:
@@ -98,7 +105,8 @@ def main() -> int:
         try:
             answer = {"value": QUESTIONS[what](*args)}
         except Exception as e:  # noqa: BLE001 - said to the one who asked
-            answer = {"error": f"{type(e).__name__}: {e}", "hip": isinstance(e, hip.HipError)}
+            of_hip = isinstance(e, hip.HipError)
+            answer = {"error": f"{type(e).__name__}: {e}", "hip": of_hip, "of_card": of_hip and e.code != _OUT_OF_MEMORY}
         print(json.dumps(answer), file=answers, flush=True)
     return 0
 

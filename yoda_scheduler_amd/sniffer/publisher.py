@@ -178,29 +178,33 @@ class SnifferAgent:
                 res[i] = {"skipped": "too little free HBM"}
                 continue
             self.probe_skipped.pop(i, None)
-            # a probe that cannot be run to its end is a failed one: what was found before it counts, and so do the
-            # cards behind
+            # a probe that cannot be run to its end is a failed one, unless the error says nothing about the card: what
+            # was found before it counts, and so do the cards behind
             got: dict = {"hip": d, "bytes": nbytes}
             try:
                 got["read_gbps"] = prober.bandwidth_gbps(d, nbytes)
                 self.measured_bw[i] = round(got["read_gbps"])
                 got["pattern_errors"] = prober.pattern_errors(d, nbytes)
             except Exception as e:  # noqa: BLE001
-                got["error"] = str(e) or repr(e)
+                got |= self._probe_error(e)
             if self.probe_matrix and "error" not in got:
                 got |= self._probe_matrix(prober, d, i, int(free_mb * self.probe_max_fraction) << 20)
             streak = self.probe_fail_streak.get(i, 0)
-            if any(got.get(k) for k in ("error", "pattern_errors", "matrix_errors")):
+            if any(got.get(k) for k in ("error_of_card", "pattern_errors", "matrix_errors")):
                 self.probe_fail_streak[i] = streak + 1
             else:
-                # a failed matrix check is only cleared by a clean one
-                self.probe_fail_streak[i] = streak if i in self._matrix_failed else 0
+                # a failed matrix check is only cleared by a clean one, and nothing by a check that was not made
+                self.probe_fail_streak[i] = streak if i in self._matrix_failed or "error" in got else 0
             self.probe_runs[i] = self.probe_runs.get(i, 0) + 1
             got["fail_streak"] = self.probe_fail_streak[i]
             res[i] = got
             if "error" in got:
                 log.warning("GPU %d: probe failed: %s", i, got["error"])
         return res
+
+    @staticmethod
+    def _probe_error(e: Exception) -> dict:
+        return {"error": str(e) or repr(e), "error_of_card": getattr(e, "of_card", True)}
 
     def _probe_matrix(self, prober, d: int, i: int, room: int) -> dict:
         """The matrix check of a card within ``room`` bytes: the fraction of the free HBM that the memory probes keep to."""
@@ -209,8 +213,10 @@ class SnifferAgent:
                 return {"matrix_skipped": "too little free HBM"}
             wrong, tflops = prober.matrix(d)
         except Exception as e:  # noqa: BLE001
-            self._matrix_failed.add(i)
-            return {"error": str(e) or repr(e)}
+            got = self._probe_error(e)
+            if got["error_of_card"]:
+                self._matrix_failed.add(i)
+            return got
         self.measured_tflops[i] = tflops
         (self._matrix_failed.add if wrong else self._matrix_failed.discard)(i)
         return {"matrix_errors": wrong, "matrix_tflops": tflops}
