@@ -297,3 +297,14 @@ def test_an_error_that_says_nothing_about_the_card_counts_for_nothing():
             w.ask(what, *args)
         assert e.value.of_card is of_card
     w.close()
+
+
+def test_a_rate_is_not_published_after_the_check_failed():
+    be = FakeBackend(1, node="n")
+    prober = FailingProber(be)
+    agent = SnifferAgent(None, "n", be, probe=True, prober=prober, probe_matrix=True)
+    agent.run_probes()
+    assert agent.build().status.card_list[0].matrix_tflops == 2500.0
+    prober.fails["matrix"] = {0: RuntimeError("hipError 700")}
+    agent.run_probes()
+    assert agent.build().status.card_list[0].matrix_tflops == 0.0

@@ -216,6 +216,7 @@ class SnifferAgent:
             got = self._probe_error(e)
             if got["error_of_card"]:
                 self._matrix_failed.add(i)
+                self.measured_tflops.pop(i, None)
             return got
         self.measured_tflops[i] = tflops
         (self._matrix_failed.add if wrong else self._matrix_failed.discard)(i)
